@@ -14,6 +14,13 @@
  * Layouts follow the reference (xiehuanyi/nanoSGLang):
  *   KV pool per layer: [num_pages, page_size, num_kv_heads, head_dim] bf16
  *     ("NHD", nano_sglang/engine/paged_kv_cache.py:60-69);
+ *   8-bit KV pool per layer (the *_fp8 cache entry points): the same shape in
+ *     e4m3 codes, plus one power-of-two scale per (token, KV head) of K and of
+ *     V as an E8M0 byte e (2^(e - 127)) in kv_scale [num_pages, num_kv_heads, 2,
+ *     page_size] (K's bytes, then V's).  A row is stored with the smallest
+ *     e >= 1 for which its largest |x| is at most 448 * 2^(e - 127), its codes
+ *     the row over that scale rounded to nearest even; a row holding a NaN, an
+ *     infinity or a value from 1.9375 * 2^127 on has e = 255 and stands for NaN;
  *   page table: CSR kv_indptr int32[B+1], kv_indices int32[nnz],
  *     kv_last_page_len int32[B] (nano_sglang/engine/engine.py:419-448);
  *   queries / outputs: [total_q, num_qo_heads, head_dim] bf16 with
@@ -43,7 +50,7 @@ enum {
 const char* nsg_last_error(void);
 /* ABI version of this header (NSG_ABI_VERSION). */
 int32_t nsg_abi_version(void);
-#define NSG_ABI_VERSION 22
+#define NSG_ABI_VERSION 23
 
 /* ------------------------------------------------------------------------
  * Verify attention: ragged multi-query attention over the paged KV cache
@@ -131,6 +138,18 @@ int32_t nsg_attn_run(const nsg_attn_plan_t* plan, const int32_t* work_d,
                      const int32_t* kv_indices, const int32_t* kv_last_page_len,
                      int32_t page_size, int32_t num_pages, float sm_scale, int32_t causal,
                      void* workspace, int64_t workspace_bytes, nsg_stream_t stream);
+
+/* nsg_attn_run over the 8-bit pool: the plans are the same (nsg_attn_plan /
+ * nsg_attn_plan_fixed), k_cache / v_cache hold e4m3 codes and kv_scale their
+ * E8M0 scales.  Q stays bf16 and unquantised, codes and scales are exact in
+ * bf16: the outputs are those of attention over the values that the pool
+ * stands for, with the probabilities rounded to bf16 after V's scale is
+ * applied.  q, out and the caches must be 16-byte aligned. */
+int32_t nsg_attn_run_fp8(const nsg_attn_plan_t* plan, const int32_t* work_d, const void* q,
+                         const void* k_cache, const void* v_cache, const void* kv_scale, void* out,
+                         const int32_t* kv_indices, int32_t page_size, int32_t num_pages,
+                         float sm_scale, int32_t causal, void* workspace,
+                         int64_t workspace_bytes, nsg_stream_t stream);
 
 /* Copies the workspace's error flags (bit 0: page id out of range) to
  * *flags_h after synchronising the stream, and clears them. */
@@ -378,6 +397,39 @@ int32_t nsg_rope_kv_write(const void* qkv, int64_t qkv_token_stride, const int64
                           int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
                           void* q_out, void* k_cache, void* v_cache, int64_t num_slots,
                           int32_t* flags, nsg_stream_t stream);
+
+/* The 8-bit pool's writes and reads; head_dim 64 or 128, page_size a power of
+ * two, num_slots = num_pages * page_size.  The slots of one write call must
+ * be distinct (a row's codes and scale are written by several threads, so two
+ * rows for one slot may mix).
+ *
+ * nsg_kv_write_fp8: nsg_kv_write into it; K and V rows ([num_kv_heads,
+ * head_dim] bf16) lie k_token_stride / v_token_stride elements apart
+ * (multiples of 8, 16-byte aligned bases).  Slots outside [0, num_slots) skip
+ * the row.
+ * nsg_rope_kv_write_fp8: nsg_rope_kv_write into it, q_out and K before
+ * quantisation bit for bit the same (qkv, q_out and the tables 16-byte
+ * aligned, qkv_token_stride a multiple of 8).
+ * nsg_kv_read_fp8: rows of the given slots as bf16, k and v [num_tokens,
+ * num_kv_heads, head_dim] contiguous: exactly the values the pool stands for
+ * (below 2^-126 those bf16 can hold); a slot outside [0, num_slots) reads as
+ * zeros. */
+int32_t nsg_kv_write_fp8(const void* k, int64_t k_token_stride, const void* v,
+                         int64_t v_token_stride, const int64_t* slots, int32_t num_tokens,
+                         void* k_cache, void* v_cache, void* kv_scale, int32_t num_kv_heads,
+                         int32_t head_dim, int32_t page_size, int64_t num_slots,
+                         nsg_stream_t stream);
+int32_t nsg_rope_kv_write_fp8(const void* qkv, int64_t qkv_token_stride,
+                              const int64_t* positions, const float* cos_table,
+                              const float* sin_table, int32_t max_position,
+                              const int64_t* slots, int32_t num_tokens, int32_t num_qo_heads,
+                              int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+                              void* q_out, void* k_cache, void* v_cache, void* kv_scale,
+                              int64_t num_slots, int32_t* flags, nsg_stream_t stream);
+int32_t nsg_kv_read_fp8(const int64_t* slots, int32_t num_tokens, const void* k_cache,
+                        const void* v_cache, const void* kv_scale, int32_t num_kv_heads,
+                        int32_t head_dim, int32_t page_size, int64_t num_slots, void* k, void* v,
+                        nsg_stream_t stream);
 
 /* Zero the K and V rows of `count` flat slots (negative slots are skipped)
  * in `num_layers` consecutive layer pools, layer_stride elements apart.

@@ -13,7 +13,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libnsg_spec.so")
 
 NSG_ATTN_WORK_INTS = 8
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 i32, i64, u32, u64, f32 = C.c_int32, C.c_int64, C.c_uint32, C.c_uint64, C.c_float
 vp = C.c_void_p
@@ -63,6 +63,12 @@ SIGNATURES = {
                                  i32, vp, vp, vp, vp, i64, vp, vp]),
     "nsg_attn_run": (i32, [C.POINTER(AttnPlan), vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32,
                            f32, i32, vp, i64, vp]),
+    "nsg_attn_run_fp8": (i32, [C.POINTER(AttnPlan), vp, vp, vp, vp, vp, vp, vp, i32, i32, f32,
+                               i32, vp, i64, vp]),
+    "nsg_kv_write_fp8": (i32, [vp, i64, vp, i64, vp, i32, vp, vp, vp, i32, i32, i32, i64, vp]),
+    "nsg_rope_kv_write_fp8": (i32, [vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, vp,
+                                    vp, vp, vp, i64, vp, vp]),
+    "nsg_kv_read_fp8": (i32, [vp, i32, vp, vp, vp, i32, i32, i32, i64, vp, vp, vp]),
     "nsg_attn_check_flags": (i32, [vp, C.POINTER(i32), vp]),
     "nsg_spec_accept_check_flags": (i32, [vp, i64, C.POINTER(i32), vp]),
     "nsg_spec_accept_greedy_tokens": (i32, [vp, vp, i64, i64, i32, i32, i32, vp, vp, vp, i32,

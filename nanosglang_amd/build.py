@@ -34,7 +34,8 @@ HIPCC_FLAGS = [
 # canonicalisation -- it doubled the cost of the per-logit max in the
 # acceptance pass.  verify_attention.hip likewise: its scores come from
 # finite Q and K (masked ones are a finite sentinel), and the canonicalising
-# maxes were 100 of the kernel's 3,240 instructions.  linear.hip, lm_head.hip: their asm copies into LDS set
+# maxes were 100 of the kernel's 3,240 instructions.  (Not so
+# the *_fp8.hip files: a row of the 8-bit pool may stand for NaN.)  linear.hip, lm_head.hip: their asm copies into LDS set
 # m0 and say so in their clobber lists, which the compiler warns about for
 # every kernel instance (the files' kernels use m0 for nothing else).
 # The files with MFMA kernels keep the accumulators in ordinary VGPRs
@@ -49,6 +50,8 @@ FILE_FLAGS = {"spec_accept.hip": ["-fno-honor-nans"],
               "linear.hip": ["-Wno-inline-asm", *MFMA_VGPR],
               "lm_head.hip": ["-Wno-inline-asm", *MFMA_VGPR],
               "ring_linear.hip": ["-Wno-inline-asm", *MFMA_VGPR],
+              "prefill_attention_fp8.hip": ["-Wno-inline-asm", *MFMA_VGPR],
+              "verify_attention_fp8.hip": ["-Wno-inline-asm", *MFMA_VGPR],
               "verify_attention.hip": ["-fno-honor-nans", *MFMA_VGPR],
               "prefill_attention.hip": ["-fno-honor-nans", "-Wno-inline-asm", *MFMA_VGPR]}
 

@@ -32,6 +32,10 @@ struct AttnParams {
   float scale_log2;
   int* flags;
   float* partials;
+  // the 8-bit pool (fp8_kv.hpp); kc and vc are then unused
+  const uint8_t* kc8;
+  const uint8_t* vc8;
+  const uint8_t* kv_scale;
 };
 
 __device__ __forceinline__ bf16x8 load_bf16x8(const bf16* p) {
@@ -92,5 +96,17 @@ __device__ __forceinline__ int swz_v(int t) {
 // 32 * waves query rows, waves = 4, or 8 at head dim 128.
 int32_t launch_prefill_attn(int head_dim, int waves, int num_work, const AttnParams& prm,
                             hipStream_t stream);
+// ... and the same over the 8-bit pool.
+int32_t launch_prefill_attn_fp8(int head_dim, int waves, int num_work, const AttnParams& prm,
+                                hipStream_t stream);
+
+// The merge of a plan's split KV ranges (verify_attention.hip); `merge` are its
+// merge items.
+int32_t launch_attn_merge(const nsg_attn_plan_t* plan, const AttnParams& prm, const int* merge,
+                          hipStream_t stream);
+
+// The verify kernel over the 8-bit pool (verify_attention_fp8.hip), without the merge.
+int32_t launch_verify_attn_fp8(const nsg_attn_plan_t* plan, const AttnParams& prm,
+                               hipStream_t stream);
 
 }  // namespace nsg

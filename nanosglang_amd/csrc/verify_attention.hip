@@ -774,6 +774,16 @@ __global__ __launch_bounds__(kThreads) void verify_merge_kernel(AttnParams p, co
 }
 
 template <int D, int RT>
+int32_t launch_merge_rt(const nsg_attn_plan_t* plan, const AttnParams& prm, const int* merge,
+                        hipStream_t stream) {
+  constexpr int kSlices = (RT * 16 * (D / 8) + kThreads - 1) / kThreads;  // a group's pieces
+  hipLaunchKernelGGL((verify_merge_kernel<D, RT>),
+                     dim3(plan->num_merge, plan->num_kv_heads, kSlices), dim3(kThreads), 0, stream,
+                     prm, merge, plan->num_merge);
+  return launch_status("verify_merge_kernel");
+}
+
+template <int D, int RT>
 int32_t launch_rt(const nsg_attn_plan_t* plan, const AttnParams& prm, const int* merge,
                   hipStream_t stream) {
   const dim3 grid(plan->num_kv_heads, plan->num_work);
@@ -788,11 +798,7 @@ int32_t launch_rt(const nsg_attn_plan_t* plan, const AttnParams& prm, const int*
   }
   int32_t rc = launch_status("verify_attn_kernel");
   if (rc || plan->num_merge == 0) return rc;
-  constexpr int kSlices = (RT * 16 * (D / 8) + kThreads - 1) / kThreads;  // a group's pieces
-  hipLaunchKernelGGL((verify_merge_kernel<D, RT>),
-                     dim3(plan->num_merge, plan->num_kv_heads, kSlices), dim3(kThreads), 0, stream,
-                     prm, merge, plan->num_merge);
-  return launch_status("verify_merge_kernel");
+  return launch_merge_rt<D, RT>(plan, prm, merge, stream);
 }
 
 template <int D>
@@ -821,7 +827,26 @@ int ilog2_exact(int v) {
   return r;
 }
 
+template <int D>
+int32_t launch_merge_d(const nsg_attn_plan_t* plan, const AttnParams& prm, const int* merge,
+                       hipStream_t stream) {
+  switch (plan->row_tiles) {
+    case 1: return launch_merge_rt<D, 1>(plan, prm, merge, stream);
+    case 2: return launch_merge_rt<D, 2>(plan, prm, merge, stream);
+    case 3: return launch_merge_rt<D, 3>(plan, prm, merge, stream);
+    case 4: return launch_merge_rt<D, 4>(plan, prm, merge, stream);
+    default: set_error("row_tiles %d out of range", plan->row_tiles); return NSG_ERR_ARG;
+  }
+}
+
 }  // namespace
+
+int32_t launch_attn_merge(const nsg_attn_plan_t* plan, const AttnParams& prm, const int* merge,
+                          hipStream_t stream) {
+  return plan->head_dim == 64 ? launch_merge_d<64>(plan, prm, merge, stream)
+                              : launch_merge_d<128>(plan, prm, merge, stream);
+}
+
 }  // namespace nsg
 
 using namespace nsg;

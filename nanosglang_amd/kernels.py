@@ -11,6 +11,10 @@ back to PyTorch or the CPU: a missing library or a non-GPU tensor raises.
 * :func:`spec_accept` -- fused acceptance / resample / bonus / rollback slots,
   replacing the loop at nano_sglang/decode/speculative.py:130-184.
 * :func:`kv_write` -- replaces the index_put scatter at causal_lm.py:335-338.
+* :func:`kv_write_fp8`, :func:`rope_kv_write_fp8`, :func:`kv_read_fp8` -- the
+  8-bit KV pool: e4m3 codes and one power-of-two scale per token and KV head;
+  the wrapper above attends to it when planned with
+  ``kv_data_type=torch.float8_e4m3fn``.
 * :func:`kv_clear_slots`, :func:`philox_uniform`.
 """
 
@@ -40,6 +44,22 @@ def _stream_ptr(device: torch.device) -> int:
 def _require_gpu(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a GPU tensor (no CPU path exists)")
+
+
+def _launch(device: torch.device, fn, what: str, *args) -> None:
+    """``fn(*args, stream)`` on ``device``'s current stream, with that device
+    current for the call."""
+    if device.index == torch.cuda.current_device():
+        check(fn(*args, _stream_ptr(device)), what)
+    else:
+        with torch.cuda.device(device):
+            check(fn(*args, _stream_ptr(device)), what)
+
+
+def _same_device(device: torch.device, **tensors: torch.Tensor | None) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -75,6 +95,29 @@ def attn_work_bound(qo_h: np.ndarray, kvp_h: np.ndarray, last_h: np.ndarray,
         L = (npg - 1) * page_size + int(last_h[b]) if npg else 0
         bound += math.ceil(ql / T) * (1 + max(1, math.ceil(L / 32)))
     return bound
+
+
+FP8 = torch.float8_e4m3fn
+
+
+def _kv_dtype(dtype) -> torch.dtype:
+    if dtype in (torch.bfloat16, "bfloat16"):
+        return torch.bfloat16
+    if dtype in (FP8, "float8_e4m3fn"):
+        return FP8
+    raise NotImplementedError(f"kv_data_type {dtype}: bfloat16 or float8_e4m3fn")
+
+
+def _check_kv_scale(kv_scale, k_cache: torch.Tensor) -> None:
+    """kv_scale of one layer's 8-bit pool k_cache (pages, P, Hkv, D)."""
+    if kv_scale is None:
+        raise ValueError("the 8-bit pool needs its kv_scale")
+    _require_gpu(kv_scale, "kv_scale")
+    N, P, Hkv, _ = k_cache.shape
+    if (kv_scale.dtype != torch.uint8 or tuple(kv_scale.shape) != (N, Hkv, 2, P)
+            or not kv_scale.is_contiguous()):
+        raise ValueError(f"kv_scale must be contiguous uint8 ({N}, {Hkv}, 2, {P}), got "
+                         f"{kv_scale.dtype} {tuple(kv_scale.shape)}")
 
 
 class BatchPrefillWithPagedKVCacheWrapper:
@@ -199,9 +242,13 @@ class BatchPrefillWithPagedKVCacheWrapper:
 
     def plan(self, qo_indptr, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len,
              num_qo_heads: int, num_kv_heads: int, head_dim_qk: int, page_size: int,
-             causal: bool = True, q_data_type=torch.bfloat16, sm_scale: float | None = None):
+             causal: bool = True, q_data_type=torch.bfloat16, sm_scale: float | None = None,
+             kv_data_type=torch.bfloat16):
+        """``kv_data_type=torch.float8_e4m3fn`` plans for the 8-bit pool
+        (:func:`kv_write_fp8`): ``run`` then takes its codes and ``kv_scale``."""
         if q_data_type not in (torch.bfloat16, "bfloat16"):
             raise NotImplementedError(f"q_data_type {q_data_type}: the kernel is bf16")
+        self._kv_dtype = _kv_dtype(kv_data_type)
         qo_h = _host_i32(qo_indptr)
         kvp_h = _host_i32(paged_kv_indptr)
         last_h = _host_i32(paged_kv_last_page_len)
@@ -242,7 +289,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
 
     def adopt_plan(self, plan: AttnPlan, total_q: int, num_qo_heads: int, num_kv_heads: int,
                    head_dim_qk: int, page_size: int, causal: bool = True,
-                   sm_scale: float | None = None) -> None:
+                   sm_scale: float | None = None, kv_data_type=torch.bfloat16) -> None:
         """Graph mode: take a plan whose metadata and work list a host routine
         (``nsg_spec_step_fill``) already wrote into this wrapper's buffers --
         the state ``plan`` leaves, without re-planning.  The plan must have the
@@ -250,6 +297,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
         ``max_kv_len``), so that a graph captured around ``run`` replays it."""
         if not self._graph:
             raise ValueError("adopt_plan is for use_cuda_graph=True wrappers")
+        self._kv_dtype = _kv_dtype(kv_data_type)
         if self._fixed is None:
             if not self._fixed_q:
                 raise ValueError("adopt_plan needs a wrapper built with max_q_len")
@@ -293,15 +341,20 @@ class BatchPrefillWithPagedKVCacheWrapper:
     def plan_info(self) -> AttnPlan:
         return self._plan
 
-    def run(self, q: torch.Tensor, paged_kv_cache, out: torch.Tensor | None = None) -> torch.Tensor:
+    def run(self, q: torch.Tensor, paged_kv_cache, out: torch.Tensor | None = None,
+            kv_scale: torch.Tensor | None = None) -> torch.Tensor:
+        """One layer: q (total_q, Hq, D) bf16, paged_kv_cache = (k_cache,
+        v_cache), each (pages, P, Hkv, D): bf16, or e4m3 codes with their
+        ``kv_scale`` (pages, Hkv, 2, P) uint8 as planned."""
         if self._plan is None:
             raise RuntimeError("run() before plan()")
         k_cache, v_cache = paged_kv_cache
         Hq, Hkv, D = self._dims
-        for name, t in (("q", q), ("k_cache", k_cache), ("v_cache", v_cache)):
+        for name, t, dt in (("q", q, torch.bfloat16), ("k_cache", k_cache, self._kv_dtype),
+                            ("v_cache", v_cache, self._kv_dtype)):
             _require_gpu(t, name)
-            if t.dtype != torch.bfloat16:
-                raise TypeError(f"{name} must be bfloat16, got {t.dtype}")
+            if t.dtype != dt:
+                raise TypeError(f"{name} must be {str(dt)[6:]}, got {t.dtype}")
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
         if tuple(q.shape) != (self._total_q, Hq, D):
@@ -310,6 +363,10 @@ class BatchPrefillWithPagedKVCacheWrapper:
                 or k_cache.shape[3] != D or v_cache.shape != k_cache.shape):
             raise ValueError(f"KV cache shape {tuple(k_cache.shape)} is not "
                              f"[pages, {self._page_size}, {Hkv}, {D}]")
+        if self._kv_dtype == FP8:
+            return self._run_fp8(q, k_cache, v_cache, kv_scale, out)
+        if kv_scale is not None:
+            raise ValueError("kv_scale is for plans with kv_data_type=torch.float8_e4m3fn")
         if out is None:
             out = torch.empty_like(q)
         rc = _lib().nsg_attn_run(
@@ -320,6 +377,21 @@ class BatchPrefillWithPagedKVCacheWrapper:
             self._ws.data_ptr(), self._ws.numel() * self._ws.element_size(),
             _stream_ptr(q.device))
         check(rc, "nsg_attn_run")
+        return out
+
+    def _run_fp8(self, q, k_cache, v_cache, kv_scale, out):
+        _check_kv_scale(kv_scale, k_cache)
+        if out is None:
+            out = torch.empty_like(q)
+        elif (out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous()):
+            raise ValueError(f"out must be contiguous bfloat16 {tuple(q.shape)}")
+        _same_device(self._device, q=q, k_cache=k_cache, v_cache=v_cache, kv_scale=kv_scale,
+                     out=out)
+        _launch(self._device, _lib().nsg_attn_run_fp8, "nsg_attn_run_fp8", C.byref(self._plan),
+                self._work_d.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                kv_scale.data_ptr(), out.data_ptr(), self._kv_indices.data_ptr(),
+                self._page_size, k_cache.shape[0], self._sm_scale, 1 if self._causal else 0,
+                self._ws.data_ptr(), self._ws.numel() * self._ws.element_size())
         return out
 
     def check_flags(self) -> int:
@@ -628,6 +700,90 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: tor
                               _stream_ptr(k.device)), "nsg_kv_write")
 
 
+def _check_fp8_pool(k_cache, v_cache, kv_scale, num_kv_heads: int, head_dim: int,
+                    device: torch.device) -> tuple[int, int]:
+    """Checks one layer's 8-bit pool; (page size, slots)."""
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t is None:
+            raise ValueError(f"{name} is missing")
+        _require_gpu(t, name)
+        if t.dtype != FP8:
+            raise TypeError(f"{name} must be float8_e4m3fn, got {t.dtype}")
+        if t.dim() != 4 or not t.is_contiguous():
+            raise ValueError(f"{name} must be one layer's contiguous (pages, P, Hkv, D) pool")
+    if v_cache.shape != k_cache.shape or tuple(k_cache.shape[2:]) != (num_kv_heads, head_dim):
+        raise ValueError(f"caches {tuple(k_cache.shape)} / {tuple(v_cache.shape)} do not match "
+                         f"(pages, P, {num_kv_heads}, {head_dim})")
+    _check_kv_scale(kv_scale, k_cache)
+    _same_device(device, k_cache=k_cache, v_cache=v_cache, kv_scale=kv_scale)
+    return k_cache.shape[1], k_cache.shape[0] * k_cache.shape[1]
+
+
+def _token_index(t, name: str, T: int, device: torch.device) -> torch.Tensor:
+    """Contiguous int64 (T,) on ``device``."""
+    _require_gpu(t, name)
+    _same_device(device, **{name: t})
+    if t.dtype not in (torch.int64, torch.int32) or t.numel() != T:
+        raise ValueError(f"{name} must hold {T} integers")
+    return t.reshape(-1).to(torch.int64).contiguous()
+
+
+def kv_write_fp8(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
+                 v_cache: torch.Tensor, kv_scale: torch.Tensor) -> None:
+    """:func:`kv_write` into the 8-bit pool (C ABI: nsg_kv_write_fp8).
+
+    k, v: (T, Hkv, D) bf16, each token's heads contiguous (views into a fused
+    projection will do); slots (T,), distinct, negative ones skip the row;
+    k_cache / v_cache: one layer's (pages, P, Hkv, D) float8_e4m3fn pool;
+    kv_scale: its (pages, Hkv, 2, P) uint8 scales, byte e for 2^(e - 127).
+    Each row is quantised by its own largest magnitude: e is the smallest for
+    which that is at most 448 * 2^(e - 127); a row with a NaN or an infinity
+    (or a value from 1.9375 * 2^127 on) reads back as NaN."""
+    _require_gpu(k, "k")
+    dev = k.device
+    if k.dim() != 3 or v.shape != k.shape:
+        raise ValueError("k and v must be (T, Hkv, D)")
+    T, Hkv, D = k.shape
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise TypeError("k and v must be bfloat16")
+    for name, t in (("k", k), ("v", v)):
+        if T and (t.stride(2) != 1 or (Hkv > 1 and t.stride(1) != D)):
+            raise ValueError(f"each row of {name} must be a contiguous (Hkv, D) block")
+    P, num_slots = _check_fp8_pool(k_cache, v_cache, kv_scale, Hkv, D, dev)
+    _same_device(dev, v=v)
+    slots = _token_index(slots, "slots", T, dev)
+    ks, vs = ((t.stride(0) if T > 1 else Hkv * D) for t in (k, v))
+    _launch(dev, _lib().nsg_kv_write_fp8, "nsg_kv_write_fp8", k.data_ptr(), ks, v.data_ptr(), vs,
+            slots.data_ptr(), T, k_cache.data_ptr(), v_cache.data_ptr(), kv_scale.data_ptr(),
+            Hkv, D, P, num_slots)
+
+
+def kv_read_fp8(slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                kv_scale: torch.Tensor, out: tuple | None = None):
+    """Rows of the 8-bit pool as bf16 (C ABI: nsg_kv_read_fp8): (k, v), each
+    (T, Hkv, D), the values the pool stands for, exactly; zeros for slots
+    outside the pool (padding)."""
+    _require_gpu(k_cache, "k_cache")
+    if k_cache.dim() != 4:
+        raise ValueError("k_cache must be one layer's (pages, P, Hkv, D) pool")
+    dev = k_cache.device
+    Hkv, D = k_cache.shape[2:]
+    P, num_slots = _check_fp8_pool(k_cache, v_cache, kv_scale, Hkv, D, dev)
+    T = slots.numel()
+    slots = _token_index(slots, "slots", T, dev)
+    if out is None:
+        out = tuple(torch.empty(T, Hkv, D, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    for t in out:
+        if t.dtype != torch.bfloat16 or tuple(t.shape) != (T, Hkv, D) or not t.is_contiguous() \
+                or t.device != dev:
+            raise ValueError(f"out must be two contiguous bfloat16 ({T}, {Hkv}, {D}) tensors "
+                             f"on {dev}")
+    _launch(dev, _lib().nsg_kv_read_fp8, "nsg_kv_read_fp8", slots.data_ptr(), T,
+            k_cache.data_ptr(), v_cache.data_ptr(), kv_scale.data_ptr(), Hkv, D, P, num_slots,
+            out[0].data_ptr(), out[1].data_ptr())
+    return out
+
+
 def kv_clear_slots(slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
     """Zero flat slots in every layer of (L, N, P, Hkv, D) pools."""
     _require_gpu(slots, "slots")
@@ -664,6 +820,48 @@ def rope_kv_write(qkv: torch.Tensor, num_qo_heads: int, num_kv_heads: int, head_
         sin_table.data_ptr(), cos_table.shape[0], _ptr(slots), T, num_qo_heads, num_kv_heads,
         head_dim, q_out.data_ptr(), _ptr(k_cache), _ptr(v_cache), num_slots, None,
         _stream_ptr(qkv.device)), "nsg_rope_kv_write")
+    return q_out
+
+
+def rope_kv_write_fp8(qkv: torch.Tensor, num_qo_heads: int, num_kv_heads: int, head_dim: int,
+                      positions: torch.Tensor, cos_table: torch.Tensor, sin_table: torch.Tensor,
+                      slots: torch.Tensor | None, k_cache: torch.Tensor | None,
+                      v_cache: torch.Tensor | None, kv_scale: torch.Tensor | None,
+                      q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`rope_kv_write` into the 8-bit pool (C ABI: nsg_rope_kv_write_fp8):
+    the same rotated q, bit for bit, and the same K rows before they are
+    quantised as :func:`kv_write_fp8` does.  ``slots`` None rotates q alone."""
+    _require_gpu(qkv, "qkv")
+    dev = qkv.device
+    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.stride(1) != 1 \
+            or qkv.shape[1] != (num_qo_heads + 2 * num_kv_heads) * head_dim:
+        raise ValueError(f"qkv must be bfloat16 (T, ({num_qo_heads} + 2 * {num_kv_heads}) * "
+                         f"{head_dim}) with unit inner stride")
+    T = qkv.shape[0]
+    for name, t in (("cos_table", cos_table), ("sin_table", sin_table)):
+        _require_gpu(t, name)
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] * 2 != head_dim \
+                or t.shape[0] != cos_table.shape[0] or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous float32 (max_position, {head_dim // 2})")
+    _same_device(dev, cos_table=cos_table, sin_table=sin_table)
+    if q_out is None:
+        q_out = torch.empty(T, num_qo_heads, head_dim, dtype=torch.bfloat16, device=dev)
+    elif q_out.dtype != torch.bfloat16 or tuple(q_out.shape) != (T, num_qo_heads, head_dim) \
+            or not q_out.is_contiguous() or q_out.device != dev:
+        raise ValueError(f"q_out must be contiguous bfloat16 ({T}, {num_qo_heads}, {head_dim}) "
+                         f"on {dev}")
+    positions = _token_index(positions, "positions", T, dev)
+    P, num_slots = 1, 0
+    if slots is not None:
+        P, num_slots = _check_fp8_pool(k_cache, v_cache, kv_scale, num_kv_heads, head_dim, dev)
+        slots = _token_index(slots, "slots", T, dev)
+    else:
+        k_cache = v_cache = kv_scale = None
+    _launch(dev, _lib().nsg_rope_kv_write_fp8, "nsg_rope_kv_write_fp8", qkv.data_ptr(),
+            qkv.stride(0) if T > 1 else qkv.shape[1], positions.data_ptr(), cos_table.data_ptr(),
+            sin_table.data_ptr(), cos_table.shape[0], _ptr(slots), T, num_qo_heads, num_kv_heads,
+            head_dim, P, q_out.data_ptr(), _ptr(k_cache), _ptr(v_cache), _ptr(kv_scale),
+            num_slots, None)
     return q_out
 
 
@@ -877,7 +1075,6 @@ def silu_mul(gate_up: torch.Tensor, out: torch.Tensor | None = None) -> torch.Te
 
 LINEAR_BIAS, LINEAR_SILU_MUL = 0, 1
 WS_FORM_MIN_WEIGHT = 16 << 20    # weights from which the *_ws entry points differ from the plain ones
-FP8 = torch.float8_e4m3fn
 
 
 def dequant_fp8(w8: torch.Tensor, w_scale: torch.Tensor) -> torch.Tensor:
