@@ -151,6 +151,74 @@ int32_t nsg_attn_run_fp8(const nsg_attn_plan_t* plan, const int32_t* work_d, con
                          float sm_scale, int32_t causal, void* workspace,
                          int64_t workspace_bytes, nsg_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Attention for a batch whose requests share the first part of their context
+ * (pages that RadixCache.match_prefix, nano_sglang/engine/radix_cache.py:68,
+ * hands to several requests): group g = requests group_indptr[g] ..
+ * group_indptr[g + 1] - 1 in the batch's order, all of them behind the prefix
+ * of pages prefix_kv_indices[prefix_kv_indptr[g] .. ) with
+ * prefix_kv_last_page_len[g] tokens on the last one (no pages: no prefix).  The
+ * CSR arrays of the batch itself describe each request's own tokens after the
+ * prefix; those hold at least its query tokens (causal), at least one token
+ * in any case.  Every query sees its whole prefix and its own tokens under
+ * the causal rule above: the result of nsg_attn_run over the concatenated
+ * page tables (whole prefix pages), computed with the prefix read once per
+ * group and query tile instead of once per request.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+  nsg_attn_plan_t own;        /* plan of the requests' own tokens             */
+  int32_t num_prefix_work;    /* work items over the prefixes                 */
+  int32_t num_merge;
+  int32_t prefix_rows;        /* rows of a prefix tile                        */
+  int32_t prefix_tile_tokens; /* query tokens of a prefix tile                */
+  int64_t prefix_partials;    /* byte offset of the prefix partials           */
+  int64_t workspace_bytes;    /* device workspace nsg_prefix_attn_run needs   */
+} nsg_prefix_attn_plan_t;
+
+/* Host-side planner, arguments as nsg_attn_plan's.  Writes own.num_work +
+ * num_prefix_work + num_merge items of NSG_ATTN_WORK_INTS int32 to work_h, which
+ * the caller copies to device memory; too small a buffer gives
+ * NSG_ERR_WORKSPACE with those counts filled in. */
+int32_t nsg_prefix_attn_plan(const int32_t* qo_indptr_h, const int32_t* group_indptr_h,
+                             int32_t num_groups, const int32_t* prefix_kv_indptr_h,
+                             const int32_t* prefix_kv_last_page_len_h,
+                             const int32_t* kv_indptr_h, const int32_t* kv_last_page_len_h,
+                             int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads,
+                             int32_t head_dim, int32_t page_size, int32_t causal,
+                             int32_t num_cus, int32_t* work_h, int32_t work_capacity,
+                             nsg_prefix_attn_plan_t* plan);
+
+/* Graph-capturable planning, as nsg_attn_fixed_capacity / nsg_attn_plan_fixed:
+ * one grid for every plan of at most `batch` requests of at most max_q_len
+ * query tokens in at most max_groups groups, each behind at most
+ * max_prefix_pages shared pages (max_kv_len bounds the own tokens, or is 0). */
+int32_t nsg_prefix_attn_fixed_capacity(int32_t batch, int32_t max_q_len, int32_t max_groups,
+                                       int32_t num_qo_heads, int32_t num_kv_heads,
+                                       int32_t head_dim, int32_t num_cus, int32_t max_kv_len,
+                                       int32_t max_prefix_pages, int32_t page_size,
+                                       int32_t* max_work, int32_t* max_prefix_work,
+                                       int32_t* max_merge);
+/* max_batch: the capacity's `batch` (the plan's own may be smaller). */
+int32_t nsg_prefix_attn_plan_fixed(
+    const int32_t* qo_indptr_h, const int32_t* group_indptr_h, int32_t num_groups,
+    const int32_t* prefix_kv_indptr_h, const int32_t* prefix_kv_last_page_len_h,
+    const int32_t* kv_indptr_h, const int32_t* kv_last_page_len_h, int32_t batch,
+    int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+    int32_t causal, int32_t num_cus, int32_t max_batch, int32_t max_q_len, int32_t max_kv_len,
+    int32_t max_work, int32_t max_prefix_work, int32_t max_merge, int32_t* work_h,
+    int32_t work_capacity, nsg_prefix_attn_plan_t* plan);
+
+/* Runs one layer over the bf16 pool (kv_scale NULL) or the 8-bit one.  work_d:
+ * device copy of the planner's list; the workspace starts with the same
+ * error-flag word as nsg_attn_run's (nsg_attn_check_flags).  q, out and the
+ * caches must be 16-byte aligned. */
+int32_t nsg_prefix_attn_run(const nsg_prefix_attn_plan_t* plan, const int32_t* work_d,
+                            const void* q, const void* k_cache, const void* v_cache,
+                            const void* kv_scale, void* out, const int32_t* prefix_kv_indices,
+                            const int32_t* kv_indices, int32_t page_size, int32_t num_pages,
+                            float sm_scale, int32_t causal, void* workspace,
+                            int64_t workspace_bytes, nsg_stream_t stream);
+
 /* Copies the workspace's error flags (bit 0: page id out of range) to
  * *flags_h after synchronising the stream, and clears them. */
 int32_t nsg_attn_check_flags(void* workspace, int32_t* flags_h, nsg_stream_t stream);

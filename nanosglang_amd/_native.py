@@ -28,6 +28,14 @@ class AttnPlan(C.Structure):
     ]
 
 
+class PrefixAttnPlan(C.Structure):
+    """Mirror of nsg_prefix_attn_plan_t."""
+    _fields_ = [
+        ("own", AttnPlan), ("num_prefix_work", i32), ("num_merge", i32), ("prefix_rows", i32),
+        ("prefix_tile_tokens", i32), ("prefix_partials", i64), ("workspace_bytes", i64),
+    ]
+
+
 class StepBufs(C.Structure):
     """Mirror of nsg_spec_step_bufs_t (host staging pointers of one step)."""
     _fields_ = [
@@ -69,6 +77,15 @@ SIGNATURES = {
     "nsg_rope_kv_write_fp8": (i32, [vp, i64, vp, vp, vp, i32, vp, i32, i32, i32, i32, i32, vp,
                                     vp, vp, vp, i64, vp, vp]),
     "nsg_kv_read_fp8": (i32, [vp, i32, vp, vp, vp, i32, i32, i32, i64, vp, vp, vp]),
+    "nsg_prefix_attn_plan": (i32, [vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32,
+                                   vp, i32, C.POINTER(PrefixAttnPlan)]),
+    "nsg_prefix_attn_fixed_capacity": (i32, [i32, i32, i32, i32, i32, i32, i32, i32, i32, i32,
+                                             C.POINTER(i32), C.POINTER(i32), C.POINTER(i32)]),
+    "nsg_prefix_attn_plan_fixed": (i32, [vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32,
+                                         i32, i32, i32, i32, i32, i32, i32, i32, vp, i32,
+                                         C.POINTER(PrefixAttnPlan)]),
+    "nsg_prefix_attn_run": (i32, [C.POINTER(PrefixAttnPlan), vp, vp, vp, vp, vp, vp, vp, vp, i32,
+                                  i32, f32, i32, vp, i64, vp]),
     "nsg_attn_check_flags": (i32, [vp, C.POINTER(i32), vp]),
     "nsg_spec_accept_check_flags": (i32, [vp, i64, C.POINTER(i32), vp]),
     "nsg_spec_accept_greedy_tokens": (i32, [vp, vp, i64, i64, i32, i32, i32, vp, vp, vp, i32,

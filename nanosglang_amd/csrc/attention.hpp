@@ -100,6 +100,15 @@ int32_t launch_prefill_attn(int head_dim, int waves, int num_work, const AttnPar
 int32_t launch_prefill_attn_fp8(int head_dim, int waves, int num_work, const AttnParams& prm,
                                 hipStream_t stream);
 
+// ... and as partial rows of a share of an item's KV range, for a merge.
+int32_t launch_prefill_part(int head_dim, int waves, int num_work, const AttnParams& prm,
+                            hipStream_t stream);
+int32_t launch_prefill_part_fp8(int head_dim, int waves, int num_work, const AttnParams& prm,
+                                hipStream_t stream);
+
+// The verify kernel over the bf16 pool without the merge (verify_attention.hip).
+int32_t launch_verify_attn(const nsg_attn_plan_t* plan, const AttnParams& prm, hipStream_t stream);
+
 // The merge of a plan's split KV ranges (verify_attention.hip); `merge` are its
 // merge items.
 int32_t launch_attn_merge(const nsg_attn_plan_t* plan, const AttnParams& prm, const int* merge,

@@ -81,7 +81,11 @@ constexpr int prefill_ring() {
 // the same LDS tiles on the way (exact: one conversion instruction per two
 // values, the scale included), once for all the workgroup's rows; the rest of
 // the kernel does not know the difference.
-template <int D, int NW, bool KV8>
+//
+// PART: an item is a share [kvb, kve) of its tile's KV range and leaves partial
+// rows (O unnormalised, m, l) of D + 4 floats for a merge, 32 NW rows per item
+// and KV head.
+template <int D, int NW, bool KV8, bool PART>
 __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(AttnParams p) {
   constexpr int KC = D / 16;              // k chunks of S^T = K Q^T
   constexpr int DT = D / 32;              // d tiles of O^T
@@ -100,6 +104,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
   const int h = blockIdx.x;
   const int* wk = p.work + (size_t)wi * NSG_ATTN_WORK_INTS;
   const int qs = wk[0], qn = wk[1], lim0 = wk[2], pb = wk[3], kve = wk[5];
+  const int kvb = PART ? wk[4] : 0;
   if (qn == 0) return;
   const int P = 1 << p.log2P;
   const int G = p.G;
@@ -110,11 +115,12 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
   const int r32 = lane & 31;
   const int g = lane >> 5;
 
-  // page ids of the item (from token 0: items are not split)
-  const int npages = min(((kve - 1) >> p.log2P) + 1, kMaxItemPages);
+  // page ids of the item
+  const int page0 = kvb >> p.log2P;
+  const int npages = min(((kve - 1) >> p.log2P) + 1 - page0, kMaxItemPages);
   bool bad_page = false;
   for (int i = tid; i < npages; i += NW * 64) {
-    int pg = p.kv_indices[pb + i];
+    int pg = p.kv_indices[pb + page0 + i];
     if ((unsigned)pg >= (unsigned)p.num_pages) {
       bad_page = true;  // reads the pool's first page instead
       pg = 0;
@@ -188,15 +194,15 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
     d_v[i] = (pc ^ swz_v<D>(t)) * 16;
     d_lds[i] = t0 * D * 2;
   }
-  const int n_it = (kve + kStep - 1) / kStep;
+  const int n_it = (kve - kvb + kStep - 1) / kStep;
   const int last_tok = kve - 1;
   auto issue = [&](int it, int slot) {
     const uint32_t sb = ring_lds + (uint32_t)slot * (2 * TILE * 2);
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       // tokens past the item's end repeat its last one (masked out)
-      const int tok = min(it * kStep + d_t[i], last_tok);
-      const int page = s_pages[min(tok >> p.log2P, kMaxItemPages - 1)];
+      const int tok = min(kvb + it * kStep + d_t[i], last_tok);
+      const int page = s_pages[min((tok >> p.log2P) - page0, kMaxItemPages - 1)];
       const size_t off = ((size_t)(uint32_t)page * P + (tok & (P - 1))) * tok_bytes;
       dma16(sb + d_lds[i], kbase + off + d_k[i]);
       dma16(sb + 2 * TILE + d_lds[i], vbase + off + d_v[i]);
@@ -211,8 +217,8 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int id = tid + i * NW * 64;
-      const int tok = min(it * kStep + id / (D / 16), last_tok);
-      const size_t page = (uint32_t)s_pages[min(tok >> p.log2P, kMaxItemPages - 1)];
+      const int tok = min(kvb + it * kStep + id / (D / 16), last_tok);
+      const size_t page = (uint32_t)s_pages[min((tok >> p.log2P) - page0, kMaxItemPages - 1)];
       const int at = tok & (P - 1);
       const size_t off = ((page * P + at) * p.Hkv + h) * D + (id % (D / 16)) * 16;
       const uint8_t* sc = p.kv_scale + ((page * p.Hkv + h) * 2 << p.log2P) + at;
@@ -375,7 +381,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
     }
     bool had = false;  // the previous step's P is pending
     for (int it = 0; it < n_it; ++it) {
-      const int t0 = it * kStep;
+      const int t0 = kvb + it * kStep;
       const bool vis = t0 <= w_hi;  // something visible to this wave's rows
       if (had) pv_mul((it - 1) & 3);
       if (vis) qk(it & 3);
@@ -407,7 +413,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
       phase();  // step `it` in LDS for every wave, the other slot free
       if (it + 1 < n_it) commit((it + 1) & 1);
       if (it + 2 < n_it) fetch(it + 2);
-      const int t0 = it * kStep;
+      const int t0 = kvb + it * kStep;
       if (t0 > w_hi) continue;
       qk(it & 1);
       softmax(t0);
@@ -426,7 +432,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
       const int cur = slot;
       if (it + kNBuf - 1 < n_it) issue(it + kNBuf - 1, slot == 0 ? kNBuf - 1 : slot - 1);
       slot = slot + 1 == kNBuf ? 0 : slot + 1;
-      const int t0 = it * kStep;
+      const int t0 = kvb + it * kStep;
       if (t0 > w_hi) continue;  // nothing visible to this wave's rows
       qk(cur);
       softmax(t0);
@@ -437,6 +443,22 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
   if (bad_page) atomicOr(p.flags, 1);
   const float l = sum_xor32(l_run);
   if (!row_ok) return;
+  if constexpr (PART) {
+    float* prow = p.partials + (((size_t)wi * p.Hkv + h) * (32 * NW) + row) * (D + 4);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const floatx16 o = oacc[dt];
+        *reinterpret_cast<floatx4*>(prow + 32 * dt + 8 * a + 4 * g) =
+            floatx4{o[4 * a], o[4 * a + 1], o[4 * a + 2], o[4 * a + 3]};
+      }
+    if (g == 0) {
+      prow[D] = m_run;
+      prow[D + 1] = l;
+    }
+    return;
+  }
   const float inv = l > 0.f ? 1.f / l : 0.f;
   bf16* orow = p.out + ((size_t)(qs + tau) * p.Hq + h * G + gam) * D + 4 * g;
 #pragma unroll
@@ -450,15 +472,16 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
     }
 }
 
-template <bool KV8>
-int32_t launch_prefill(int head_dim, int waves, int num_work, const AttnParams& prm, hipStream_t stream) {
+template <bool KV8, bool PART>
+int32_t launch_prefill(int head_dim, int waves, int num_work, const AttnParams& prm,
+                       hipStream_t stream) {
   const dim3 grid(prm.Hkv, num_work), block(waves * 64);
   if (head_dim == 64 && waves == 4)
-    hipLaunchKernelGGL((prefill_attn_kernel<64, 4, KV8>), grid, block, 0, stream, prm);
+    hipLaunchKernelGGL((prefill_attn_kernel<64, 4, KV8, PART>), grid, block, 0, stream, prm);
   else if (head_dim == 128 && waves == 4)
-    hipLaunchKernelGGL((prefill_attn_kernel<128, 4, KV8>), grid, block, 0, stream, prm);
+    hipLaunchKernelGGL((prefill_attn_kernel<128, 4, KV8, PART>), grid, block, 0, stream, prm);
   else if (head_dim == 128 && waves == 8)
-    hipLaunchKernelGGL((prefill_attn_kernel<128, 8, KV8>), grid, block, 0, stream, prm);
+    hipLaunchKernelGGL((prefill_attn_kernel<128, 8, KV8, PART>), grid, block, 0, stream, prm);
   else {
     set_error("prefill attention: head_dim %d, %d waves", head_dim, waves);
     return NSG_ERR_ARG;

@@ -7,7 +7,11 @@ namespace nsg {
 
 int32_t launch_prefill_attn_fp8(int head_dim, int waves, int num_work, const AttnParams& prm,
                                 hipStream_t stream) {
-  return launch_prefill<true>(head_dim, waves, num_work, prm, stream);
+  return launch_prefill<true, false>(head_dim, waves, num_work, prm, stream);
+}
+int32_t launch_prefill_part_fp8(int head_dim, int waves, int num_work, const AttnParams& prm,
+                                 hipStream_t stream) {
+  return launch_prefill<true, true>(head_dim, waves, num_work, prm, stream);
 }
 
 }  // namespace nsg

@@ -1,0 +1,427 @@
+// Attention for a batch whose requests share the first part of their context:
+// groups of consecutive requests, each with one prefix on shared pages, then
+// every request's own tokens on its own pages.
+//
+//   o_r = sum over prefix and own tokens of softmax(sm_scale q_r . k) v,
+//
+// the prefix visible to every row of its group, the own part under the
+// bottom-right causal rule (nano_sglang/model/causal_lm.py:359-471 over the
+// concatenated context; the shared pages are what RadixCache.match_prefix,
+// nano_sglang/engine/radix_cache.py:68, hands to several requests).
+//
+// The prefix is attended to once per group: its query tiles run over the
+// group's packed query tokens as if they were one request, so K and V of the
+// prefix are read once per tile of up to 256 rows instead of once per request,
+// and a decode step's few rows per request fill MFMA tiles together.  Three
+// launches: the own parts and the prefix tiles leave partial rows (O, m, l; the
+// kernels of verify_attention.hip and prefill_attention.hpp, over shares of the
+// KV range), the merge below joins a row's partials of both.
+#include <algorithm>
+#include <vector>
+
+#include "attention.hpp"
+
+namespace nsg {
+namespace {
+
+constexpr int64_t kHeader = 256;   // workspace: flags word + padding
+constexpr int kThreads = 256;
+constexpr int kBatch = 8;          // partial rows whose loads a merge thread has in flight
+constexpr int kAll = 0x3fffffff;   // causal limit of prefix tiles: everything is visible
+constexpr int kStep = 64;          // shares of a prefix are whole steps of this many tokens
+constexpr int kMinSteps = 4;       // ... at least this many
+
+struct MergeParams {
+  const int* merge;
+  const float* own;      // partial rows of the own parts, own_rows per item and KV head
+  const float* prefix;   // ... of the prefix tiles
+  bf16* out;
+  int own_rows, prefix_rows, prefix_tokens;  // rows per item; query tokens per prefix tile
+  int Hq, Hkv, G;
+};
+
+// Merge item: [first query token, query tokens, first own item, own splits,
+// the group's first prefix item, its splits, its first query token, -].  A
+// thread owns 8 columns of a row and folds up to kBatch partials per memory
+// round trip.
+template <int D>
+__global__ __launch_bounds__(kThreads) void prefix_merge_kernel(MergeParams p) {
+  constexpr int PSTRIDE = D + 4;
+  constexpr int CH = D / 8;
+  const int* mw = p.merge + (size_t)blockIdx.x * NSG_ATTN_WORK_INTS;
+  const int qs = mw[0], qn = mw[1], wi0 = mw[2], ns = mw[3], pw0 = mw[4], pns = mw[5];
+  const int item = (int)blockIdx.z * kThreads + (int)threadIdx.x;
+  if (item >= qn * p.G * CH) return;  // (a padding item has no query tokens)
+  const int h = blockIdx.y;
+  const int row = item / CH;
+  const int c0 = (item - row * CH) * 8;
+  const int tau = row / p.G;
+  const int gam = row - tau * p.G;
+  const int at = qs + tau - mw[6];  // the token's place in its group
+  const int tile = at / p.prefix_tokens;
+  const int prow = (at - tile * p.prefix_tokens) * p.G + gam;
+  const float* own = p.own + (((size_t)wi0 * p.Hkv + h) * p.own_rows + row) * PSTRIDE;
+  const size_t own_step = (size_t)p.Hkv * p.own_rows * PSTRIDE;
+  const float* pre =
+      p.prefix + (((size_t)(pw0 + tile * pns) * p.Hkv + h) * p.prefix_rows + prow) * PSTRIDE;
+  const size_t pre_step = (size_t)p.Hkv * p.prefix_rows * PSTRIDE;
+  float M = kMaskVal, lsum = 0.f;
+  float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const int n = ns + pns;
+  for (int s0 = 0; s0 < n; s0 += kBatch) {
+    floatx4 ml[kBatch], a[kBatch], b[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {  // past the last: re-reads it
+      const int s = min(s0 + j, n - 1);
+      const float* r = s < ns ? own + s * own_step : pre + (s - ns) * pre_step;
+      ml[j] = *reinterpret_cast<const floatx4*>(r + D);
+      a[j] = *reinterpret_cast<const floatx4*>(r + c0);
+      b[j] = *reinterpret_cast<const floatx4*>(r + c0 + 4);
+    }
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (s0 + j >= n) break;
+      const float Mn = fmaxf(M, ml[j][0]);
+      const float sc = __builtin_amdgcn_exp2f(M - Mn);
+      const float wt = __builtin_amdgcn_exp2f(ml[j][0] - Mn);
+      lsum = lsum * sc + wt * ml[j][1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o[i] = o[i] * sc + wt * a[j][i];
+        o[4 + i] = o[4 + i] * sc + wt * b[j][i];
+      }
+      M = Mn;
+    }
+  }
+  const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);
+  bf16* orow = p.out + ((size_t)(qs + tau) * p.Hq + h * p.G + gam) * D + c0;
+  *reinterpret_cast<u32x4*>(orow) =
+      u32x4{cvt_pk_bf16(o[0] * inv, o[1] * inv), cvt_pk_bf16(o[2] * inv, o[3] * inv),
+            cvt_pk_bf16(o[4] * inv, o[5] * inv), cvt_pk_bf16(o[6] * inv, o[7] * inv)};
+}
+
+// Rows of a prefix tile for groups of at most `rows` rows: the verify kernel's
+// 16-row tiles up to 64, the prefill kernel's 128 or (head dim 128) 256 beyond.
+int prefix_rows(int64_t rows, int head_dim) {
+  if (rows <= 64) return (int)std::max<int64_t>(16, (rows + 15) / 16 * 16);
+  return rows <= 128 || head_dim == 64 ? 128 : 256;
+}
+
+// Prefix items aimed at: the workgroups that the GPU holds at once.
+int prefix_target(int rows, int head_dim, int num_cus, int num_kv_heads) {
+  const int per_cu = rows <= 64 ? 3 : rows == 256 ? 1 : head_dim == 64 ? 3 : 2;
+  return std::max(1, num_cus * per_cu / num_kv_heads);
+}
+
+struct Sizes {
+  bool fixed;
+  int max_batch, max_q_len, max_kv_len, max_work, max_prefix_work, max_merge;
+};
+
+int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
+                  const int32_t* pkv, const int32_t* plast, const int32_t* kvp,
+                  const int32_t* last, int32_t batch, int32_t Hq, int32_t Hkv, int32_t head_dim,
+                  int32_t page_size, int32_t causal, int32_t num_cus, const Sizes& sz,
+                  int32_t* work_h, int32_t work_capacity, nsg_prefix_attn_plan_t* plan) {
+  NSG_CHECK_ARG(plan && qo && groups && pkv && plast && kvp && last, "null argument");
+  NSG_CHECK_ARG(batch >= 0 && num_groups >= 0, "batch %d, %d groups", batch, num_groups);
+  NSG_CHECK_ARG(groups[0] == 0 && groups[num_groups] == batch,
+                "group_indptr must run from 0 to the batch (%d), has %d .. %d", batch, groups[0],
+                groups[num_groups]);
+  NSG_CHECK_ARG(pkv[0] == 0, "prefix_kv_indptr must start at 0");
+  if (num_cus <= 0) num_cus = 256;
+  // ---- the own parts: an attention plan whose items all leave partials ----
+  std::vector<int32_t> own(1024 * NSG_ATTN_WORK_INTS);
+  nsg_attn_plan_t op{};
+  for (;;) {
+    const int32_t cap = (int32_t)(own.size() / NSG_ATTN_WORK_INTS);
+    const int32_t rc =
+        sz.fixed ? nsg_attn_plan_fixed(qo, kvp, last, batch, Hq, Hkv, head_dim, page_size, causal,
+                                       num_cus, sz.max_q_len, sz.max_kv_len, sz.max_work,
+                                       sz.max_merge, own.data(), cap, &op)
+                 : nsg_attn_plan(qo, kvp, last, batch, Hq, Hkv, head_dim, page_size, causal,
+                                 num_cus, own.data(), cap, &op);
+    if (rc == NSG_OK) break;
+    // (a fixed list that is too small stays so whatever the buffer)
+    const bool grow = rc == NSG_ERR_WORKSPACE &&
+                      (sz.fixed ? cap < sz.max_work + sz.max_merge : cap < (1 << 22));
+    if (!grow) return rc;
+    own.resize(own.size() * 4);
+  }
+  const int G = Hq / Hkv;
+  // ---- the prefix tiles ----
+  int64_t most = 0;
+  for (int g = 0; g < num_groups; ++g) {
+    NSG_CHECK_ARG(groups[g] <= groups[g + 1], "group %d: decreasing group_indptr", g);
+    const int np = pkv[g + 1] - pkv[g];
+    NSG_CHECK_ARG(np >= 0, "group %d: decreasing prefix_kv_indptr", g);
+    NSG_CHECK_ARG(np == 0 || (plast[g] >= 1 && plast[g] <= page_size),
+                  "group %d: prefix last_page_len %d outside [1, %d]", g, plast[g], page_size);
+    NSG_CHECK_ARG(np <= kAll / page_size, "group %d: prefix of %d pages", g, np);
+    most = std::max<int64_t>(most, (int64_t)(qo[groups[g + 1]] - qo[groups[g]]) * G);
+  }
+  if (sz.fixed) most = (int64_t)sz.max_batch * sz.max_q_len * G;
+  const int rows = prefix_rows(most, head_dim);
+  const int T = std::max(1, rows / G);
+  auto prefix_len = [&](int g) {
+    const int np = pkv[g + 1] - pkv[g];
+    return np ? (np - 1) * page_size + plast[g] : 0;
+  };
+  auto tiles_of = [&](int g) { return (qo[groups[g + 1]] - qo[groups[g]] + T - 1) / T; };
+  int64_t total = 0;
+  for (int g = 0; g < num_groups; ++g)
+    total += (int64_t)tiles_of(g) * ((prefix_len(g) + kStep - 1) / kStep);
+  const int target = prefix_target(rows, head_dim, num_cus, Hkv);
+  int64_t chunk = std::max<int64_t>(kMinSteps, (total + target - 1) / target);
+  // an item's page ids must fit the kernels' list
+  chunk = std::min(chunk, std::max<int64_t>(1, (int64_t)(kMaxItemPages - 2) * page_size / kStep));
+  std::vector<int32_t> pre;
+  std::vector<int> first(num_groups), splits(num_groups);
+  for (int g = 0; g < num_groups; ++g) {
+    const int len = prefix_len(g), tiles = tiles_of(g), q0 = qo[groups[g]], q1 = qo[groups[g + 1]];
+    const int64_t steps = (len + kStep - 1) / kStep;
+    const int ns = (int)((steps + chunk - 1) / chunk);
+    first[g] = (int)(pre.size() / NSG_ATTN_WORK_INTS);
+    splits[g] = ns;
+    for (int t = 0; t < tiles; ++t)
+      for (int s = 0; s < ns; ++s) {
+        const int b = (int)(steps * s / ns) * kStep, e = (int)(steps * (s + 1) / ns) * kStep;
+        pre.insert(pre.end(), {q0 + t * T, std::min(T, q1 - q0 - t * T), kAll, pkv[g], b,
+                               std::min(len, e), 2, 0});
+      }
+  }
+  const int n_pre = (int)(pre.size() / NSG_ATTN_WORK_INTS);
+  if (sz.fixed && n_pre > sz.max_prefix_work) {
+    set_error("plan needs %d prefix items, the fixed list holds %d", n_pre, sz.max_prefix_work);
+    return NSG_ERR_WORKSPACE;
+  }
+  // ---- merge items: one per query tile of the own parts, whose splits are
+  //      consecutive items ----
+  std::vector<int32_t> merge;
+  int g = 0;
+  for (int i = 0; i < op.num_work;) {
+    int32_t* w = own.data() + (size_t)i * NSG_ATTN_WORK_INTS;
+    if (w[1] == 0) break;  // padding
+    const int ns = std::max(1, w[6]);
+    for (int s = 0; s < ns; ++s) w[(size_t)s * NSG_ATTN_WORK_INTS + 6] = std::max(2, ns);
+    // (tiles need not come in the requests' order)
+    g = (int)(std::upper_bound(groups, groups + num_groups + 1, 0,
+                               [&](int, int32_t b) { return qo[b] > w[0]; }) -
+              groups) - 1;
+    merge.insert(merge.end(), {w[0], w[1], i, ns, first[g], splits[g], qo[groups[g]], 0});
+    i += ns;
+  }
+  const int n_merge = (int)(merge.size() / NSG_ATTN_WORK_INTS);
+  plan->own = op;
+  plan->num_prefix_work = sz.fixed ? sz.max_prefix_work : n_pre;
+  plan->num_merge = sz.fixed ? sz.max_merge : n_merge;
+  plan->prefix_rows = rows;
+  plan->prefix_tile_tokens = T;
+  const int64_t row_bytes = (int64_t)Hkv * (head_dim + 4) * 4;
+  plan->prefix_partials = kHeader + (int64_t)op.num_work * op.row_tiles * 16 * row_bytes;
+  plan->workspace_bytes = plan->prefix_partials + (int64_t)plan->num_prefix_work * rows * row_bytes;
+  const int64_t items = (int64_t)op.num_work + plan->num_prefix_work + plan->num_merge;
+  if (sz.fixed && n_merge > sz.max_merge) {
+    set_error("plan needs %d merge items, the fixed list holds %d", n_merge, sz.max_merge);
+    return NSG_ERR_WORKSPACE;
+  }
+  if (!work_h || items > work_capacity) {
+    set_error("work list needs %lld items, buffer holds %d", (long long)items, work_capacity);
+    return NSG_ERR_WORKSPACE;
+  }
+  auto put = [&](const std::vector<int32_t>& from, int n, int slots) {
+    std::copy(from.begin(), from.begin() + (size_t)n * NSG_ATTN_WORK_INTS, work_h);
+    std::fill(work_h + (size_t)n * NSG_ATTN_WORK_INTS, work_h + (size_t)slots * NSG_ATTN_WORK_INTS,
+              0);
+    work_h += (size_t)slots * NSG_ATTN_WORK_INTS;
+  };
+  put(own, op.num_work, op.num_work);
+  put(pre, n_pre, plan->num_prefix_work);
+  put(merge, n_merge, plan->num_merge);
+  clear_error();
+  return NSG_OK;
+}
+
+template <typename F>
+int32_t guarded(F&& f) {  // no C++ exception crosses the C ABI
+  try {
+    return f();
+  } catch (...) {
+    set_error("out of host memory while planning");
+    return NSG_ERR_ARG;
+  }
+}
+
+}  // namespace
+}  // namespace nsg
+
+using namespace nsg;
+
+extern "C" int32_t nsg_prefix_attn_plan(
+    const int32_t* qo_indptr_h, const int32_t* group_indptr_h, int32_t num_groups,
+    const int32_t* prefix_kv_indptr_h, const int32_t* prefix_kv_last_page_len_h,
+    const int32_t* kv_indptr_h, const int32_t* kv_last_page_len_h, int32_t batch,
+    int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+    int32_t causal, int32_t num_cus, int32_t* work_h, int32_t work_capacity,
+    nsg_prefix_attn_plan_t* plan) {
+  return guarded([&] {
+    return plan_impl(qo_indptr_h, group_indptr_h, num_groups, prefix_kv_indptr_h,
+                     prefix_kv_last_page_len_h, kv_indptr_h, kv_last_page_len_h, batch,
+                     num_qo_heads, num_kv_heads, head_dim, page_size, causal, num_cus, Sizes{},
+                     work_h, work_capacity, plan);
+  });
+}
+
+extern "C" int32_t nsg_prefix_attn_fixed_capacity(int32_t batch, int32_t max_q_len,
+                                                  int32_t max_groups, int32_t num_qo_heads,
+                                                  int32_t num_kv_heads, int32_t head_dim,
+                                                  int32_t num_cus, int32_t max_kv_len,
+                                                  int32_t max_prefix_pages, int32_t page_size,
+                                                  int32_t* max_work, int32_t* max_prefix_work,
+                                                  int32_t* max_merge) {
+  NSG_CHECK_ARG(max_work && max_prefix_work && max_merge, "null argument");
+  NSG_CHECK_ARG(max_groups >= 1 && max_prefix_pages >= 0 && page_size >= 1,
+                "max_groups %d, max_prefix_pages %d, page_size %d", max_groups, max_prefix_pages,
+                page_size);
+  NSG_CHECK_ARG(head_dim == 64 || head_dim == 128, "head_dim %d (64 or 128)", head_dim);
+  if (int32_t rc = nsg_attn_fixed_capacity(batch, max_q_len, num_qo_heads, num_kv_heads, num_cus,
+                                           max_kv_len, max_work, max_merge))
+    return rc;
+  if (num_cus <= 0) num_cus = 256;
+  const int G = num_qo_heads / num_kv_heads;
+  const int64_t rows_all = (int64_t)batch * max_q_len * G;
+  const int rows = prefix_rows(rows_all, head_dim);
+  const int T = std::max(1, rows / G);
+  // tiles: one more per group for its last, partly filled one; shares: the
+  // target, one more per tile for rounding, or what an item's page list forces
+  const int64_t tiles = ((int64_t)batch * max_q_len + T - 1) / T + max_groups;
+  const int64_t steps = ((int64_t)max_prefix_pages * page_size + kStep - 1) / kStep;
+  const int64_t by_pages =
+      std::max<int64_t>(1, (int64_t)(kMaxItemPages - 2) * page_size / kStep);
+  const int64_t forced = tiles * ((steps + by_pages - 1) / by_pages);
+  const int64_t n = std::max(forced, prefix_target(rows, head_dim, num_cus, num_kv_heads) + tiles);
+  NSG_CHECK_ARG(n <= 1 << 24, "too many prefix items (%lld)", (long long)n);
+  *max_prefix_work = (int32_t)n;
+  *max_merge = *max_work;  // every query tile of the own parts meets its prefix
+  clear_error();
+  return NSG_OK;
+}
+
+extern "C" int32_t nsg_prefix_attn_plan_fixed(
+    const int32_t* qo_indptr_h, const int32_t* group_indptr_h, int32_t num_groups,
+    const int32_t* prefix_kv_indptr_h, const int32_t* prefix_kv_last_page_len_h,
+    const int32_t* kv_indptr_h, const int32_t* kv_last_page_len_h, int32_t batch,
+    int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim, int32_t page_size,
+    int32_t causal, int32_t num_cus, int32_t max_batch, int32_t max_q_len, int32_t max_kv_len,
+    int32_t max_work, int32_t max_prefix_work, int32_t max_merge, int32_t* work_h,
+    int32_t work_capacity, nsg_prefix_attn_plan_t* plan) {
+  NSG_CHECK_ARG(max_prefix_work >= 0, "max_prefix_work %d", max_prefix_work);
+  NSG_CHECK_ARG(batch <= max_batch, "batch %d exceeds the fixed plan's %d", batch, max_batch);
+  return guarded([&] {
+    return plan_impl(qo_indptr_h, group_indptr_h, num_groups, prefix_kv_indptr_h,
+                     prefix_kv_last_page_len_h, kv_indptr_h, kv_last_page_len_h, batch,
+                     num_qo_heads, num_kv_heads, head_dim, page_size, causal, num_cus,
+                     Sizes{true, max_batch, max_q_len, max_kv_len, max_work, max_prefix_work, max_merge},
+                     work_h, work_capacity, plan);
+  });
+}
+
+extern "C" int32_t nsg_prefix_attn_run(const nsg_prefix_attn_plan_t* plan, const int32_t* work_d,
+                                       const void* q, const void* k_cache, const void* v_cache,
+                                       const void* kv_scale, void* out,
+                                       const int32_t* prefix_kv_indices,
+                                       const int32_t* kv_indices, int32_t page_size,
+                                       int32_t num_pages, float sm_scale, int32_t causal,
+                                       void* workspace, int64_t workspace_bytes,
+                                       nsg_stream_t stream) {
+  NSG_CHECK_ARG(plan != nullptr, "null plan");
+  if (plan->own.num_work == 0) {
+    clear_error();
+    return NSG_OK;
+  }
+  NSG_CHECK_ARG(work_d && q && k_cache && v_cache && out && kv_indices && workspace &&
+                    (prefix_kv_indices || plan->num_prefix_work == 0),
+                "null pointer argument");
+  NSG_CHECK_ARG(page_size > 0 && (page_size & (page_size - 1)) == 0,
+                "page_size %d must be a power of two", page_size);
+  NSG_CHECK_ARG(num_pages > 0, "num_pages %d", num_pages);
+  NSG_CHECK_ARG(sm_scale > 0.f, "sm_scale %g must be positive", (double)sm_scale);
+  NSG_CHECK_ARG(((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)q | (uintptr_t)out) % 16 == 0,
+                "q, out and the caches must be 16-byte aligned");
+  const nsg_attn_plan_t& own = plan->own;
+  if (own.head_dim != 64 && own.head_dim != 128) {
+    set_error("head_dim %d not supported", own.head_dim);
+    return NSG_ERR_UNSUPPORTED;
+  }
+  NSG_CHECK_ARG(own.kv_groups == 1 || page_size >= 16,
+                "page_size %d: the plan's %d KV groups need pages of 16+ tokens (plan and run "
+                "with the same page size)", page_size, own.kv_groups);
+  if (workspace_bytes < plan->workspace_bytes) {
+    set_error("workspace has %lld bytes, plan needs %lld", (long long)workspace_bytes,
+              (long long)plan->workspace_bytes);
+    return NSG_ERR_WORKSPACE;
+  }
+  const bool fp8 = kv_scale != nullptr;
+  char* ws = static_cast<char*>(workspace);
+  AttnParams prm{};
+  prm.q = static_cast<const bf16*>(q);
+  prm.kc = static_cast<const bf16*>(k_cache);
+  prm.vc = static_cast<const bf16*>(v_cache);
+  prm.kc8 = static_cast<const uint8_t*>(k_cache);
+  prm.vc8 = static_cast<const uint8_t*>(v_cache);
+  prm.kv_scale = static_cast<const uint8_t*>(kv_scale);
+  prm.out = static_cast<bf16*>(out);
+  prm.Hq = own.num_qo_heads;
+  prm.Hkv = own.num_kv_heads;
+  prm.G = own.num_qo_heads / own.num_kv_heads;
+  prm.log2P = __builtin_ctz((unsigned)page_size);
+  prm.num_pages = num_pages;
+  prm.causal = causal ? 1 : 0;
+  prm.scale_log2 = sm_scale * 1.4426950408889634f;
+  prm.flags = reinterpret_cast<int*>(ws);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  auto launch = [&](const nsg_attn_plan_t& pl) {
+    if (pl.row_tiles >= 8)
+      return (fp8 ? launch_prefill_part_fp8 : launch_prefill_part)(pl.head_dim, pl.row_tiles / 2,
+                                                                   pl.num_work, prm, s);
+    return (fp8 ? launch_verify_attn_fp8 : launch_verify_attn)(&pl, prm, s);
+  };
+  // own parts
+  prm.work = work_d;
+  prm.num_work = own.num_work;
+  prm.kv_indices = kv_indices;
+  prm.partials = reinterpret_cast<float*>(ws + kHeader);
+  if (int32_t rc = launch(own)) return rc;
+  // prefix tiles
+  const int* work_p = work_d + (size_t)own.num_work * NSG_ATTN_WORK_INTS;
+  if (plan->num_prefix_work > 0) {
+    nsg_attn_plan_t pp = own;
+    pp.num_work = plan->num_prefix_work;
+    pp.row_tiles = plan->prefix_rows / 16;
+    pp.kv_groups = 1;
+    prm.work = work_p;
+    prm.num_work = pp.num_work;
+    prm.kv_indices = prefix_kv_indices;
+    prm.partials = reinterpret_cast<float*>(ws + plan->prefix_partials);
+    if (int32_t rc = launch(pp)) return rc;
+  }
+  MergeParams m{};
+  m.merge = work_p + (size_t)plan->num_prefix_work * NSG_ATTN_WORK_INTS;
+  m.own = reinterpret_cast<const float*>(ws + kHeader);
+  m.prefix = reinterpret_cast<const float*>(ws + plan->prefix_partials);
+  m.out = prm.out;
+  m.own_rows = own.row_tiles * 16;
+  m.prefix_rows = plan->prefix_rows;
+  m.prefix_tokens = plan->prefix_tile_tokens;
+  m.Hq = prm.Hq;
+  m.Hkv = prm.Hkv;
+  m.G = prm.G;
+  const unsigned slices =
+      (unsigned)((own.q_tile_tokens * prm.G * (own.head_dim / 8) + kThreads - 1) / kThreads);
+  const dim3 grid(plan->num_merge, prm.Hkv, slices);
+  if (own.head_dim == 64)
+    hipLaunchKernelGGL(prefix_merge_kernel<64>, grid, dim3(kThreads), 0, s, m);
+  else
+    hipLaunchKernelGGL(prefix_merge_kernel<128>, grid, dim3(kThreads), 0, s, m);
+  return launch_status("prefix_merge_kernel");
+}

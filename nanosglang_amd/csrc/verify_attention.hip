@@ -841,6 +841,14 @@ int32_t launch_merge_d(const nsg_attn_plan_t* plan, const AttnParams& prm, const
 
 }  // namespace
 
+int32_t launch_verify_attn(const nsg_attn_plan_t* plan, const AttnParams& prm,
+                           hipStream_t stream) {
+  nsg_attn_plan_t unmerged = *plan;
+  unmerged.num_merge = 0;
+  return plan->head_dim == 64 ? launch_d<64>(&unmerged, prm, nullptr, stream)
+                              : launch_d<128>(&unmerged, prm, nullptr, stream);
+}
+
 int32_t launch_attn_merge(const nsg_attn_plan_t* plan, const AttnParams& prm, const int* merge,
                           hipStream_t stream) {
   return plan->head_dim == 64 ? launch_merge_d<64>(plan, prm, merge, stream)

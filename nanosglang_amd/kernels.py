@@ -8,6 +8,9 @@ back to PyTorch or the CPU: a missing library or a non-GPU tensor raises.
   wrapper the reference uses for paged attention (constructed at
   nano_sglang/engine/engine.py:106-108, planned at engine.py:451-462, run at
   nano_sglang/model/causal_lm.py:340).
+* :class:`SharedPrefixAttentionWrapper` -- the same attention for groups of
+  requests that share the first part of their context, that part attended to
+  once per group.
 * :func:`spec_accept` -- fused acceptance / resample / bonus / rollback slots,
   replacing the loop at nano_sglang/decode/speculative.py:130-184.
 * :func:`kv_write` -- replaces the index_put scatter at causal_lm.py:335-338.
@@ -28,7 +31,7 @@ import numpy as np
 import torch
 
 from . import _native
-from ._native import NSG_ATTN_WORK_INTS, AttnPlan, check
+from ._native import NSG_ATTN_WORK_INTS, AttnPlan, PrefixAttnPlan, check
 
 MI355X_CUS = 256
 
@@ -396,6 +399,206 @@ class BatchPrefillWithPagedKVCacheWrapper:
 
     def check_flags(self) -> int:
         """Synchronises and returns (then clears) the kernel's error flags."""
+        f = C.c_int32(0)
+        check(_lib().nsg_attn_check_flags(self._ws.data_ptr(), C.byref(f),
+                                          _stream_ptr(self._device)), "nsg_attn_check_flags")
+        return f.value
+
+
+class SharedPrefixAttentionWrapper:
+    """Paged attention for a batch whose requests share the first part of their
+    context (a system prompt, a document, several samples of one prompt).
+
+    >>> w = SharedPrefixAttentionWrapper(workspace_u8)
+    >>> w.plan(qo_indptr, group_indptr, prefix_kv_indptr, prefix_kv_indices,
+    ...        prefix_kv_last_page_len, kv_indptr, kv_indices, kv_last_page_len,
+    ...        num_qo_heads, num_kv_heads, head_dim, page_size)
+    >>> out = w.run(q, (k_cache[layer], v_cache[layer]))
+
+    Group g is requests ``group_indptr[g] .. group_indptr[g + 1] - 1``; its prefix
+    is a CSR row of pages (none: no prefix), the batch's CSR arrays describe each
+    request's own tokens after it.  The outputs are those of
+    :class:`BatchPrefillWithPagedKVCacheWrapper` over the joined contexts; the
+    prefix is read once per group and tile of up to 256 query rows.  Meant for
+    decode and verify steps; prompts run too, with partial rows of every query
+    in the workspace.
+
+    ``plan`` works on the host, ``run`` enqueues on the current stream of the
+    workspace's device and never syncs.  With ``use_cuda_graph=True`` the buffers
+    have fixed addresses and one grid serves every plan of at most ``max_batch``
+    requests of ``max_q_len`` query tokens, ``max_groups`` groups,
+    ``max_prefix_pages`` pages per prefix and ``max_pages`` own pages in all, so a
+    graph captured around ``run`` replays after each re-plan (``max_kv_len`` > 0
+    bounds a request's own tokens, and then they are never split); a plan of
+    fewer query rows leaves the rest of ``out`` as it was.  Without it a captured
+    ``run`` keeps the plan it was captured with."""
+
+    def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD",
+                 num_cus: int = MI355X_CUS, use_cuda_graph: bool = False,
+                 max_batch: int | None = None, max_q_len: int | None = None,
+                 max_groups: int = 1, max_prefix_pages: int | None = None,
+                 max_pages: int | None = None, max_kv_len: int = 0):
+        if kv_layout != "NHD":
+            raise ValueError(f"kv_layout {kv_layout!r}: only 'NHD'")
+        _require_gpu(float_workspace_buffer, "workspace")
+        self._ws = float_workspace_buffer
+        self._ws.zero_()
+        self._ws_bytes = self._ws.numel() * self._ws.element_size()
+        self._device = self._ws.device
+        self._num_cus = num_cus
+        self._plan: PrefixAttnPlan | None = None
+        self._graph = bool(use_cuda_graph)
+        self._sizes = None
+        if self._graph:
+            if None in (max_batch, max_q_len, max_prefix_pages, max_pages):
+                raise ValueError("use_cuda_graph=True needs max_batch, max_q_len, "
+                                 "max_prefix_pages and max_pages")
+            self._sizes = (int(max_batch), int(max_q_len), int(max_groups),
+                           int(max_prefix_pages), int(max_kv_len))
+            self._caps = None
+            self._fixed_shape = None
+            self._idx = torch.zeros(max(1, int(max_pages)), dtype=torch.int32,
+                                    device=self._device)
+            self._pidx = torch.zeros(max(1, int(max_prefix_pages) * int(max_groups)),
+                                     dtype=torch.int32, device=self._device)
+        # index and work arrays of plans that a graph captured: it reads them
+        # for as long as it lives
+        self._captured: list = []
+
+    def plan(self, qo_indptr, group_indptr, prefix_kv_indptr, prefix_kv_indices,
+             prefix_kv_last_page_len, paged_kv_indptr, paged_kv_indices, paged_kv_last_page_len,
+             num_qo_heads: int, num_kv_heads: int, head_dim_qk: int, page_size: int,
+             causal: bool = True, q_data_type=torch.bfloat16, sm_scale: float | None = None,
+             kv_data_type=torch.bfloat16) -> None:
+        if q_data_type not in (torch.bfloat16, "bfloat16"):
+            raise NotImplementedError(f"q_data_type {q_data_type}: the kernel is bf16")
+        kv_dtype = _kv_dtype(kv_data_type)
+        qo, grp, pptr, plast, ptr, last = map(_host_i32, (
+            qo_indptr, group_indptr, prefix_kv_indptr, prefix_kv_last_page_len, paged_kv_indptr,
+            paged_kv_last_page_len))
+        B, n = len(qo) - 1, len(grp) - 1
+        if B < 0 or n < 0 or len(ptr) != B + 1 or len(last) != B or len(pptr) != n + 1 \
+                or len(plast) != n:
+            raise ValueError("qo_indptr, group_indptr, the kv_indptr and last_page_len arrays "
+                             "disagree on batch or groups")
+        idx, pidx = _host_i32(paged_kv_indices), _host_i32(prefix_kv_indices)
+        if len(idx) < ptr[-1] or len(pidx) < pptr[-1]:
+            raise ValueError(f"{len(idx)} / {len(pidx)} page ids, the indptr arrays end at "
+                             f"{ptr[-1]} / {pptr[-1]}")
+        idx, pidx = idx[:ptr[-1]], pidx[:pptr[-1]]
+        lib = _lib()
+        pl = PrefixAttnPlan()
+        args = (qo.ctypes.data, grp.ctypes.data, n, pptr.ctypes.data, plast.ctypes.data,
+                ptr.ctypes.data, last.ctypes.data, B, num_qo_heads, num_kv_heads, head_dim_qk,
+                page_size, 1 if causal else 0, self._num_cus)
+        if self._graph:
+            work = self._plan_fixed(lib, pl, args, n, idx, pidx)
+        else:
+            cap = 256
+            while True:
+                work = np.zeros(cap * NSG_ATTN_WORK_INTS, np.int32)
+                rc = lib.nsg_prefix_attn_plan(*args, work.ctypes.data, cap, C.byref(pl))
+                need = pl.own.num_work + pl.num_prefix_work + pl.num_merge
+                if rc == 3 and need > cap:
+                    cap = need
+                    continue
+                check(rc, "nsg_prefix_attn_plan")
+                break
+            self._check_ws(pl)
+            work = work[:need * NSG_ATTN_WORK_INTS]
+            self._work, self._idx, self._pidx = (
+                torch.from_numpy(x if len(x) else np.zeros(1, np.int32)).to(self._device)
+                for x in (work, idx, pidx))
+        self._plan = pl
+        self._kv_dtype = kv_dtype
+        self._total_q = int(qo[-1])
+        self._dims = (num_qo_heads, num_kv_heads, head_dim_qk)
+        self._page_size = page_size
+        self._causal = bool(causal)
+        self._sm_scale = (1.0 / math.sqrt(head_dim_qk)) if sm_scale is None else float(sm_scale)
+
+    def _check_ws(self, pl: PrefixAttnPlan) -> None:
+        if pl.workspace_bytes > self._ws_bytes:
+            raise RuntimeError(f"attention workspace too small: plan needs {pl.workspace_bytes} "
+                               f"bytes, buffer has {self._ws_bytes}")
+
+    def _plan_fixed(self, lib, pl, args, n_groups, idx, pidx) -> None:
+        mb, mq, mg, mp, mk = self._sizes
+        Hq, Hkv, D, P = args[8:12]
+        if self._caps is None:
+            c = [C.c_int32(0) for _ in range(3)]
+            check(lib.nsg_prefix_attn_fixed_capacity(mb, mq, mg, Hq, Hkv, D, self._num_cus, mk,
+                                                     mp, P, *map(C.byref, c)),
+                  "nsg_prefix_attn_fixed_capacity")
+            # (the page list is in pages of this size: one shape per wrapper)
+            self._caps, self._fixed_shape = [x.value for x in c], (Hq, Hkv, D, P)
+            self._work_h = np.zeros((sum(self._caps)) * NSG_ATTN_WORK_INTS, np.int32)
+            self._work = torch.zeros(len(self._work_h), dtype=torch.int32, device=self._device)
+        if (Hq, Hkv, D, P) != self._fixed_shape:
+            raise ValueError(f"graph-mode wrapper holds heads and pages {self._fixed_shape}, "
+                             f"plan has {(Hq, Hkv, D, P)}")
+        if n_groups > mg or len(pidx) > self._pidx.numel() or len(idx) > self._idx.numel():
+            raise ValueError(f"{n_groups} groups, {len(pidx)} prefix and {len(idx)} own pages "
+                             f"exceed the buffers ({mg}, {self._pidx.numel()}, "
+                             f"{self._idx.numel()})")
+        check(lib.nsg_prefix_attn_plan_fixed(*args, mb, mq, mk, *self._caps,
+                                             self._work_h.ctypes.data, sum(self._caps),
+                                             C.byref(pl)), "nsg_prefix_attn_plan_fixed")
+        self._check_ws(pl)
+        self._work.copy_(torch.from_numpy(self._work_h))
+        for buf, h in ((self._idx, idx), (self._pidx, pidx)):
+            if len(h):
+                buf[:len(h)].copy_(torch.from_numpy(h))
+
+    @property
+    def plan_info(self) -> PrefixAttnPlan:
+        return self._plan
+
+    def run(self, q: torch.Tensor, paged_kv_cache, out: torch.Tensor | None = None,
+            kv_scale: torch.Tensor | None = None) -> torch.Tensor:
+        """One layer, arguments as
+        :meth:`BatchPrefillWithPagedKVCacheWrapper.run`'s; in graph mode q and
+        out may have more rows than the plan."""
+        if self._plan is None:
+            raise RuntimeError("run() before plan()")
+        k_cache, v_cache = paged_kv_cache
+        Hq, Hkv, D = self._dims
+        for name, t, dt in (("q", q, torch.bfloat16), ("k_cache", k_cache, self._kv_dtype),
+                            ("v_cache", v_cache, self._kv_dtype)):
+            _require_gpu(t, name)
+            if t.dtype != dt:
+                raise TypeError(f"{name} must be {str(dt)[6:]}, got {t.dtype}")
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+        if q.dim() != 3 or tuple(q.shape[1:]) != (Hq, D) or not (
+                q.shape[0] == self._total_q or (self._graph and q.shape[0] > self._total_q)):
+            raise ValueError(f"q shape {tuple(q.shape)} != planned {(self._total_q, Hq, D)}")
+        if (k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (self._page_size, Hkv, D)
+                or v_cache.shape != k_cache.shape):
+            raise ValueError(f"KV cache shape {tuple(k_cache.shape)} is not "
+                             f"[pages, {self._page_size}, {Hkv}, {D}]")
+        if self._kv_dtype == FP8:
+            _check_kv_scale(kv_scale, k_cache)
+        elif kv_scale is not None:
+            raise ValueError("kv_scale is for plans with kv_data_type=torch.float8_e4m3fn")
+        if out is None:
+            out = torch.empty_like(q)
+        elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous():
+            raise ValueError(f"out must be contiguous bfloat16 {tuple(q.shape)}")
+        _same_device(self._device, q=q, k_cache=k_cache, v_cache=v_cache, kv_scale=kv_scale,
+                     out=out)
+        if not self._graph and torch.cuda.is_current_stream_capturing():
+            self._captured.append((self._work, self._idx, self._pidx))
+        _launch(self._device, _lib().nsg_prefix_attn_run, "nsg_prefix_attn_run",
+                C.byref(self._plan), self._work.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
+                v_cache.data_ptr(), _ptr(kv_scale), out.data_ptr(), self._pidx.data_ptr(),
+                self._idx.data_ptr(), self._page_size, k_cache.shape[0], self._sm_scale,
+                1 if self._causal else 0, self._ws.data_ptr(), self._ws_bytes)
+        return out
+
+    def check_flags(self) -> int:
+        """Synchronises and returns (then clears) the kernels' error flags (bit
+        0: a page id out of range)."""
         f = C.c_int32(0)
         check(_lib().nsg_attn_check_flags(self._ws.data_ptr(), C.byref(f),
                                           _stream_ptr(self._device)), "nsg_attn_check_flags")
