@@ -349,6 +349,8 @@ extern "C" int32_t nsg_prefix_attn_run(const nsg_prefix_attn_plan_t* plan, const
   NSG_CHECK_ARG(((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)q | (uintptr_t)out) % 16 == 0,
                 "q, out and the caches must be 16-byte aligned");
   const nsg_attn_plan_t& own = plan->own;
+  NSG_CHECK_ARG((int64_t)page_size * own.num_kv_heads * own.head_dim < 1ll << 31,
+                "a page of %d tokens is too large", page_size);
   if (own.head_dim != 64 && own.head_dim != 128) {
     set_error("head_dim %d not supported", own.head_dim);
     return NSG_ERR_UNSUPPORTED;

@@ -56,18 +56,25 @@ __device__ __forceinline__ int swz8_v(int t) {
 // copy in flight before each LDS read, does not see these; the ring's own
 // waits order them.  Lane l lands at lds + 16 l (codes), lds + 4 l (a scale
 // byte, zero-extended).  NT: no reuse expected.
+// Source: a wave-uniform base plus 32 bits a lane, or a lane's own address.
 template <bool NT>
-__device__ __forceinline__ void dma_codes(uint32_t lds, const uint8_t* src) {
+__device__ __forceinline__ void dma_codes(uint32_t lds, uint64_t base, uint32_t off) {
   if constexpr (NT)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
                  :
-                 : "s"(lds), "v"(src)
+                 : "s"(lds), "v"(off), "s"(base)
                  : "memory", "m0");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
-                 : "s"(lds), "v"(src)
+                 : "s"(lds), "v"(off), "s"(base)
                  : "memory", "m0");
+}
+__device__ __forceinline__ void dma_codes(uint32_t lds, const uint8_t* src) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds), "v"(src)
+               : "memory", "m0");
 }
 __device__ __forceinline__ void dma_scale(uint32_t lds, const uint8_t* src) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off"
@@ -114,16 +121,23 @@ __global__ __launch_bounds__(RT * KS * 64) void verify_attn_fp8_kernel(AttnParam
   const int r16 = lane & 15;
   const int g4 = lane >> 4;
 
-  const int page0 = kvb >> p.log2P;
-  const int npages = kve > kvb ? ((kve - 1) >> p.log2P) - page0 + 1 : 0;
-  for (int i = tid; i < min(npages, kListPages); i += NTHR) s_pages[i] = p.kv_indices[pb + page0 + i];
-
   // this group's share of the item's steps
   const int n_all = (kve - kvb + kTok - 1) / kTok;
   const int per = (n_all + KS - 1) / KS;
   const int n_it = max(0, min(per, n_all - grp * per));
   const int gkvb = kvb + grp * per * kTok;
   const int last_tok = kve - 1;
+
+  // Page ids: a step takes one a lane (of token t0 + lane).  Those of the first
+  // steps come straight from memory, beside Q; the item's list goes to LDS for
+  // the later ones.
+  const int page0 = kvb >> p.log2P;
+  const int npages = kve > kvb ? (last_tok >> p.log2P) - page0 + 1 : 0;
+  int vp[NBUF - 1];
+#pragma unroll
+  for (int it = 0; it < NBUF - 1; ++it)
+    vp[it] = n_it ? p.kv_indices[pb + (min(gkvb + it * kTok + lane, last_tok) >> p.log2P)] : 0;
+  int list_id = per > NBUF - 1 && tid < npages ? p.kv_indices[pb + page0 + tid] : 0;
 
   // this lane's query row and its causal limit (rows past the tile's end load
   // its first row, all their scores masked)
@@ -141,7 +155,6 @@ __global__ __launch_bounds__(RT * KS * 64) void verify_attn_fp8_kernel(AttnParam
   }
 #pragma unroll
   for (int c = 0; c < KC; ++c) asm volatile("" ::"v"(__builtin_bit_cast(u32x4, qf[c])));
-  __syncthreads();  // page ids visible
 
   floatx4 oacc[DT];
 #pragma unroll
@@ -151,38 +164,58 @@ __global__ __launch_bounds__(RT * KS * 64) void verify_attn_fp8_kernel(AttnParam
 
   const uint32_t ring0 = __builtin_amdgcn_readfirstlane(lds_addr(ring) + grp * (NBUF * SLOT));
   const uint8_t* gring = ring + grp * (NBUF * SLOT);
-  const size_t tok_bytes = (size_t)p.Hkv * D;
-  auto page_of = [&](int tok) {
-    const int i = (tok >> p.log2P) - page0;
-    int pg = i < kListPages ? s_pages[i] : p.kv_indices[pb + page0 + i];
+  const uint32_t tok_bytes = (uint32_t)(p.Hkv * D);
+  const uint32_t page_bytes = tok_bytes << p.log2P;  // (below 2^31: checked at the entry point)
+  const uint32_t scale_bytes = (uint32_t)(2 * p.Hkv) << p.log2P;
+  // A lane's source offset inside a block of TPI token rows, for K and V
+  // (block 0; the swizzles of block `blk` differ in one bit), and its scale's.
+  const int tr = lane / CPR, pc = lane % CPR;
+  const uint32_t row_off = (uint32_t)tr * tok_bytes;
+  const uint32_t koff0 = row_off + (pc ^ swz8_k<D>(tr)) * 16;
+  const uint32_t voff0 = row_off + (pc ^ swz8_v<D>(tr)) * 16;
+  const uint8_t* sbase = p.kv_scale + ((size_t)(2 * h) << p.log2P);
+  // This wave's copies of step `it` into slot `slot`, given its page ids.
+  auto issue = [&](int it, int slot, int pg) {
+    const int t0 = gkvb + it * kTok;
+    const uint32_t sb = ring0 + (uint32_t)slot * SLOT;
     if ((unsigned)pg >= (unsigned)p.num_pages) {
       bad_page = true;  // reads the pool's first page instead
       pg = 0;
     }
-    return (uint32_t)pg;
-  };
-  // This wave's copies of step `it` into slot `slot`; tokens past the item's
-  // end repeat its last one (masked out).
-  auto issue = [&](int it, int slot) {
-    const int t0 = gkvb + it * kTok;
-    const uint32_t sb = ring0 + (uint32_t)slot * SLOT;
+    if (P >= TPI && t0 + kTok <= kve) {
+      // a block's rows lie on one page: scalar addresses
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int blk = (wave + RT * i) % NBLK;  // (a padding copy repeats a real one)
-      const int t = blk * TPI + lane / CPR;
-      const int tok = min(t0 + t, last_tok);
-      const size_t off = ((size_t)page_of(tok) * P + (tok & (P - 1))) * tok_bytes + (size_t)h * D;
-      const int pc = lane % CPR;
-      const uint32_t dst = sb + blk * (TPI * D);
-      dma_codes<KS == 1>(dst, p.kc8 + off + (pc ^ swz8_k<D>(t)) * 16);
-      dma_codes<KS == 1>(dst + TILE, p.vc8 + off + (pc ^ swz8_v<D>(t)) * 16);
+      for (int i = 0; i < NB; ++i) {
+        const int blk = (wave + RT * i) % NBLK;  // (a padding copy repeats a real one)
+        const uint32_t page = (uint32_t)__builtin_amdgcn_readlane(pg, blk * TPI);
+        const uint64_t off = (uint64_t)page * page_bytes +
+                             (uint32_t)((t0 + blk * TPI) & (P - 1)) * tok_bytes + (uint32_t)(h * D);
+        const uint32_t dst = sb + blk * (TPI * D);
+        dma_codes<KS == 1>(dst, (uint64_t)p.kc8 + off, koff0 ^ ((swz8_k<D>(blk * TPI)) * 16));
+        dma_codes<KS == 1>(dst + TILE, (uint64_t)p.vc8 + off, voff0 ^ ((swz8_v<D>(blk * TPI)) * 16));
+      }
+    } else {
+      // small pages, or the item's last step, where tokens past the end
+      // repeat the last one (masked out)
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int blk = (wave + RT * i) % NBLK;
+        const int t = blk * TPI + tr;
+        const int tok = min(t0 + t, last_tok);
+        const uint32_t page = (uint32_t)__shfl(pg, t);
+        const size_t off = (size_t)page * page_bytes + (uint32_t)(tok & (P - 1)) * tok_bytes +
+                           (uint32_t)(h * D);
+        const uint32_t dst = sb + blk * (TPI * D);
+        dma_codes(dst, p.kc8 + off + (pc ^ swz8_k<D>(t)) * 16);
+        dma_codes(dst + TILE, p.vc8 + off + (pc ^ swz8_v<D>(t)) * 16);
+      }
     }
     const int tok = min(t0 + lane, last_tok);
-    const size_t so = (((size_t)page_of(tok) * p.Hkv + h) * 2 << p.log2P) + (tok & (P - 1));
+    const uint8_t* so = sbase + (size_t)(uint32_t)pg * scale_bytes + (tok & (P - 1));
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       const int which = RT == 1 ? i : wave & 1;
-      dma_scale(sb + 2 * TILE + which * (kTok * 4), p.kv_scale + so + ((size_t)which << p.log2P));
+      dma_scale(sb + 2 * TILE + which * (kTok * 4), so + ((size_t)which << p.log2P));
     }
   };
 
@@ -197,9 +230,31 @@ __global__ __launch_bounds__(RT * KS * 64) void verify_attn_fp8_kernel(AttnParam
   const int voff = vt * D + 8 * (r16 & 1);
   const int vswz = swz8_v<D>(vt);
 
+  // (all ids have landed before any copy is issued: the compiler's wait for
+  // one of them would otherwise drain the copies)
+#pragma unroll
+  for (int it = 0; it < NBUF - 1; ++it) asm volatile("" ::"v"(vp[it]));
+  asm volatile("" : "+v"(list_id));
 #pragma unroll
   for (int it = 0; it < NBUF - 1; ++it)
-    if (it < n_it) issue(it, it);
+    if (it < n_it) issue(it, it, vp[it]);
+  // the page list, where there are later steps (the same for every wave)
+  const bool long_list = npages > kListPages;
+  if (per > NBUF - 1) {
+    if (tid < kListPages) s_pages[tid] = list_id;
+    for (int i = tid + NTHR; i < min(npages, kListPages); i += NTHR)
+      s_pages[i] = p.kv_indices[pb + page0 + i];
+    __syncthreads();
+  }
+  auto step_pages = [&](int it) {
+    const int i = (min(gkvb + it * kTok + lane, last_tok) >> p.log2P) - page0;
+    int pg = s_pages[min(i, kListPages - 1)];
+    // (kept apart from the load below: one load from either address would be a
+    // flat load, whose wait drains the ring)
+    asm volatile("" : "+v"(pg));
+    if (long_list && i >= kListPages) pg = p.kv_indices[pb + page0 + i];
+    return pg;
+  };
 
   const int n_loop = RT == 1 ? n_it : per;  // groups of several waves keep their barriers matched
   int slot = 0;
@@ -213,7 +268,8 @@ __global__ __launch_bounds__(RT * KS * 64) void verify_attn_fp8_kernel(AttnParam
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
     }
-    if (it + NBUF - 1 < n_it) issue(it + NBUF - 1, slot == 0 ? NBUF - 1 : slot - 1);
+    if (it + NBUF - 1 < n_it)
+      issue(it + NBUF - 1, slot == 0 ? NBUF - 1 : slot - 1, step_pages(it + NBUF - 1));
     const uint8_t* Kt = gring + slot * SLOT;
     slot = slot + 1 == NBUF ? 0 : slot + 1;
     if (!real) continue;
@@ -439,6 +495,8 @@ extern "C" int32_t nsg_attn_run_fp8(const nsg_attn_plan_t* plan, const int32_t* 
                 "page_size %d must be a power of two", page_size);
   NSG_CHECK_ARG(num_pages > 0, "num_pages %d", num_pages);
   NSG_CHECK_ARG(sm_scale > 0.f, "sm_scale %g must be positive", (double)sm_scale);
+  NSG_CHECK_ARG((int64_t)page_size * plan->num_kv_heads * plan->head_dim < 1ll << 31,
+                "a page of %d tokens is too large", page_size);
   NSG_CHECK_ARG(((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)q | (uintptr_t)out) % 16 == 0,
                 "q, out and the caches must be 16-byte aligned");
   if (plan->head_dim != 64 && plan->head_dim != 128) {
