@@ -284,7 +284,16 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
     mx = max_xor32(mx);
     mx = (MASKED && mx == kMaskVal) ? kMaskVal : mx * p.scale_log2;
     const bool grow = mx > m_run + kLazyRescale;
-    if (__builtin_amdgcn_ballot_w64(grow)) {
+    if constexpr (KV8 || PART) {
+      // (always: around a branch the compiler keeps two copies of the
+      // accumulators, moves one to the other whichever way it goes, and spills)
+      const float mnew = grow ? mx : m_run;
+      const float alpha = __builtin_amdgcn_exp2f(m_run - mnew);
+      m_run = mnew;
+      l_run *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
+    } else if (__builtin_amdgcn_ballot_w64(grow)) {
       const float mnew = grow ? mx : m_run;
       const float alpha = __builtin_amdgcn_exp2f(m_run - mnew);
       m_run = mnew;
@@ -393,7 +402,9 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
       const int nx = it + 2 + grp;
       if constexpr (KV8) {
         if (nx < n_it) commit(nx & 3);
+        __builtin_amdgcn_sched_barrier(0);
         if (nx + 1 < n_it) fetch(nx + 1);
+        __builtin_amdgcn_sched_barrier(0);
       } else {
         if (nx < n_it) issue(nx, nx & 3);
       }
@@ -412,7 +423,9 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
     for (int it = 0; it < n_it; ++it) {
       phase();  // step `it` in LDS for every wave, the other slot free
       if (it + 1 < n_it) commit((it + 1) & 1);
+      __builtin_amdgcn_sched_barrier(0);
       if (it + 2 < n_it) fetch(it + 2);
+      __builtin_amdgcn_sched_barrier(0);
       const int t0 = kvb + it * kStep;
       if (t0 > w_hi) continue;
       qk(it & 1);
