@@ -171,6 +171,8 @@ typedef struct {
   int32_t num_merge;
   int32_t prefix_rows;        /* rows of a prefix tile                        */
   int32_t prefix_tile_tokens; /* query tokens of a prefix tile                */
+  int32_t prefix_kv_groups;   /* KV groups per prefix workgroup               */
+  int32_t merge_lanes;        /* lanes that share a row's partials            */
   int64_t prefix_partials;    /* byte offset of the prefix partials           */
   int64_t workspace_bytes;    /* device workspace nsg_prefix_attn_run needs   */
 } nsg_prefix_attn_plan_t;

@@ -32,7 +32,8 @@ class PrefixAttnPlan(C.Structure):
     """Mirror of nsg_prefix_attn_plan_t."""
     _fields_ = [
         ("own", AttnPlan), ("num_prefix_work", i32), ("num_merge", i32), ("prefix_rows", i32),
-        ("prefix_tile_tokens", i32), ("prefix_partials", i64), ("workspace_bytes", i64),
+        ("prefix_tile_tokens", i32), ("prefix_kv_groups", i32), ("merge_lanes", i32),
+        ("prefix_partials", i64), ("workspace_bytes", i64),
     ]
 
 

@@ -50,7 +50,8 @@ FILE_FLAGS = {"spec_accept.hip": ["-fno-honor-nans"],
               "linear.hip": ["-Wno-inline-asm", *MFMA_VGPR],
               "lm_head.hip": ["-Wno-inline-asm", *MFMA_VGPR],
               "ring_linear.hip": ["-Wno-inline-asm", *MFMA_VGPR],
-              "prefill_attention_fp8.hip": ["-Wno-inline-asm", *MFMA_VGPR],
+              "prefill_tiles.hip": ["-fno-honor-nans", "-Wno-inline-asm", *MFMA_VGPR],
+              "prefill_tiles_fp8.hip": ["-Wno-inline-asm", *MFMA_VGPR],
               "verify_attention_fp8.hip": ["-Wno-inline-asm", *MFMA_VGPR],
               "verify_attention.hip": ["-fno-honor-nans", *MFMA_VGPR],
               "prefill_attention.hip": ["-fno-honor-nans", "-Wno-inline-asm", *MFMA_VGPR]}

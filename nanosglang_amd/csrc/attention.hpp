@@ -92,19 +92,28 @@ __device__ __forceinline__ int swz_v(int t) {
 }
 
 
+// The attention planner behind nsg_attn_plan (fixed_work < 0) and
+// nsg_attn_plan_fixed (its max_work, max_merge, max_q_len, max_kv_len); regime: 1
+// several KV groups per workgroup, 0 one, -1 the planner's own choice.
+int32_t plan_attn(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
+                  const int32_t* kv_last_page_len_h, int32_t batch, int32_t num_qo_heads,
+                  int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int32_t causal,
+                  int32_t num_cus, int32_t* work_h, int32_t work_capacity, int32_t fixed_work,
+                  int32_t fixed_merge, int32_t fixed_q_len, int32_t fixed_kv_len, int32_t regime,
+                  nsg_attn_plan_t* plan);
+
 // The prefill kernel (prefill_attention.hip): unsplit work items of up to
 // 32 * waves query rows, waves = 4, or 8 at head dim 128.
 int32_t launch_prefill_attn(int head_dim, int waves, int num_work, const AttnParams& prm,
                             hipStream_t stream);
-// ... and the same over the 8-bit pool.
+// The same tiles over the 8-bit pool, and over either pool as partial rows of a
+// share of an item's KV range, for a merge (prefill_tiles.hpp).
 int32_t launch_prefill_attn_fp8(int head_dim, int waves, int num_work, const AttnParams& prm,
                                 hipStream_t stream);
-
-// ... and as partial rows of a share of an item's KV range, for a merge.
-int32_t launch_prefill_part(int head_dim, int waves, int num_work, const AttnParams& prm,
-                            hipStream_t stream);
-int32_t launch_prefill_part_fp8(int head_dim, int waves, int num_work, const AttnParams& prm,
-                                hipStream_t stream);
+int32_t launch_tiles_part(int head_dim, int waves, int num_work, const AttnParams& prm,
+                          hipStream_t stream);
+int32_t launch_tiles_part_fp8(int head_dim, int waves, int num_work, const AttnParams& prm,
+                              hipStream_t stream);
 
 // The verify kernel over the bf16 pool without the merge (verify_attention.hip).
 int32_t launch_verify_attn(const nsg_attn_plan_t* plan, const AttnParams& prm, hipStream_t stream);

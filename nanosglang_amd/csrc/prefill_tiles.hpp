@@ -1,37 +1,24 @@
-// Prefill attention for gfx950 (included by prefill_attention.hip for the bf16
-// pool and prefill_attention_fp8.hip for the 8-bit one, which are compiled with
-// different flags): the work items of a plan whose query tiles
-// are full (prompts: every position is a query), same semantics and inputs
-// as the verify kernel (verify_attention.hip): ragged multi-query attention
-// over the NHD paged KV cache, GQA, bottom-right causal rule
-// (nano_sglang/model/causal_lm.py:359-471).
+// The prefill kernel (prefill_attention.hip: 32 query rows a wave on
+// v_mfma_f32_32x32x16_bf16, 64-token steps through an LDS ring) for what that one
+// does not do:
+//   KV8   the 8-bit pool (fp8_kv.hpp).  A thread loads 16-byte runs of codes
+//         and their row's scale bytes a step ahead and turns the present ones
+//         into bf16 in the same LDS tiles on the way, exactly, one instruction
+//         per two values, once for all of the workgroup's rows.
+//   PART  an item is a share [kvb, kve) of its tile's KV range and leaves partial
+//         rows (O unnormalised, m, l) of D + 4 floats for a merge, 32 NW rows per
+//         item and KV head.
 //
-// What bounds it: the matrix cores and, beside them, one exponential per
-// score.  A wave therefore owns 32 query rows (v_mfma_f32_32x32x16_bf16): a
-// K or V fragment read from LDS feeds 32 rows instead of the verify kernel's
-// 16, and a workgroup of NW waves (32 NW rows of one request and KV head)
-// shares each K / V step, so LDS and L2 reads per flop are halved and
-// quartered.  No KV split: the planner takes this kernel only for enough well
-// filled tiles, so there is no merge launch either.
-//
-// Per workgroup, in 64-token steps through an LDS ring filled by DMA:
-//   * S^T = K Q^T (M = 32 tokens, N = 32 query rows): lane l holds row l % 32
-//     and 16 tokens 8 a + 4 (l / 32) + b of each 32-token half, so a row's max
-//     and sum need one swap between the wave's halves;
-//   * P^T in bf16 is directly the B operand of O^T += V^T P^T: the MFMA's k
-//     slots (l / 32, j) stand for tokens 4 (l / 32) + j and 8 + 4 (l / 32) +
-//     j - 4 of 16, and the V^T fragments are read in that order by
-//     ds_read_b64_tr_b16;
-//   * online softmax in base 2 with lazy rescaling, as in the verify kernel;
-//     steps wholly above a wave's causal limits are skipped, steps wholly
-//     below them run without the mask.
-//
-// Measured (eager calls, the verify kernel before): two prompts of 2048 - 8192
-// tokens, 32 / 8 heads of 128: 1092 -> 607 us (0.92 PFLOP/s of the causal
-// products; all waves in step 671 - 696, raised wave priority in the matrix
-// phase 631); 32 prompts of 100 - 512, 14 / 2 heads of 64: 37.1 -> 20.1 us.
-// At head dim 128 the counters show the matrix cores busy 36 % and the vector
-// ALU 47 % of the time, LDS 28 %, a third of its cycles bank conflicts.
+// Softmax may subtract any base from a row's scores, so a row keeps the maximum
+// of its item's first step (a row that sees nothing of it sees nothing of the
+// item): the steps after it need no maximum, no rescaling of the accumulators
+// and no wait for either.  Later scores above the base make probabilities above
+// one, which bf16 and the fp32 sums hold with the same relative error up to
+// 2^127; a workgroup one of whose rows passed 2^60 finds its rows' maxima in a
+// pass over K and goes through its steps once more.  Dropping the running maximum
+// (16 max3, a swap, 64 multiplies or, around a branch, as many register moves of
+// the accumulators per step) measured at 4 x 1000-token chunks over 2048 - 8192,
+// 32 / 8 heads of 128, from 413 to 386 us (0.74 PFLOP/s of the causal products).
 #pragma once
 
 #include "attention.hpp"
@@ -65,40 +52,32 @@ __device__ __forceinline__ float sum_xor32(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Ring slots.  Head dim 128: four with the two wave groups (a slot is read over
-// four phases), two for 128 rows (68 KB: two workgroups a CU).  Head dim 64:
-// three (52 KB: three workgroups of four waves a CU, at 168 registers).
-// Over the 8-bit pool a step waits in registers, so two slots do where the wave
-// groups do not alternate.
+// Ring slots.  Two wave groups (head dim 128, 8 waves): four, a slot is read
+// over four phases.  Otherwise two of head dim 128 (68 KB, two workgroups a CU)
+// or three of 64 (52 KB, three a CU); the 8-bit pool's next step waits in
+// registers, so two do.
 template <int D, int NW, bool KV8>
-constexpr int prefill_ring() {
+constexpr int tile_ring() {
   if (NW == 8) return 4;
-  return D == 64 && !KV8 ? 3 : 2;
+  if (KV8) return 2;
+  return D == 64 ? 3 : 2;
 }
 
-// KV8: the 8-bit pool.  A thread loads 16-byte runs of codes and their row's
-// scales for the step after next, and turns those of the next one into bf16 in
-// the same LDS tiles on the way (exact: one conversion instruction per two
-// values, the scale included), once for all the workgroup's rows; the rest of
-// the kernel does not know the difference.
-//
-// PART: an item is a share [kvb, kve) of its tile's KV range and leaves partial
-// rows (O unnormalised, m, l) of D + 4 floats for a merge, 32 NW rows per item
-// and KV head.
 template <int D, int NW, bool KV8, bool PART>
-__global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(AttnParams p) {
+__global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void attn_tile_kernel(AttnParams p) {
   constexpr int KC = D / 16;              // k chunks of S^T = K Q^T
   constexpr int DT = D / 32;              // d tiles of O^T
-  constexpr int CPR = D / 8;              // 16-byte chunks per token row
+  constexpr int CPR = D / 8;              // 16-byte chunks per token row of a tile
   constexpr int TILE = kStep * D;         // bf16 per K (or V) tile
   constexpr int TPI = 64 / CPR;           // token rows per 1 KB copy
   constexpr int NR = kStep / TPI / NW;    // row blocks a wave copies per step (K and V each)
   constexpr int NI = 2 * NR;              // copies per wave per step
-  constexpr int kNBuf = prefill_ring<D, NW, KV8>();
-  constexpr bool PP = NW == 8;              // (head dim 128 only) two wave groups half a step apart
-  static_assert(NR >= 1 && (kNBuf - 1) * NI <= 63, "vmcnt counts to 63");
-  __shared__ __attribute__((aligned(1024))) bf16 ring[kNBuf][2][TILE];
+  constexpr int NBUF = tile_ring<D, NW, KV8>();
+  constexpr bool PP = NW == 8;            // (head dim 128 only) two wave groups half a step apart
+  static_assert(NR >= 1 && (NBUF - 1) * NI <= 63, "vmcnt counts to 63");
+  __shared__ __attribute__((aligned(1024))) bf16 ring[NBUF][2][TILE];
   __shared__ int s_pages[kMaxItemPages];
+  __shared__ int s_redo;  // some row's base was too low
 
   const int wi = blockIdx.y;
   const int h = blockIdx.x;
@@ -127,6 +106,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
     }
     s_pages[i] = pg;
   }
+  if (tid == 0) s_redo = 0;
 
   // this lane's query row and its causal limit; the wave's smallest and
   // largest limit (rows past the tile's end load its first row, masked out)
@@ -152,20 +132,14 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
   __syncthreads();  // page ids visible
 
   floatx16 oacc[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) oacc[dt][i] = 0.f;
   float m_run = kMaskVal, l_run = 0.f;
 
   // LDS read offsets (bytes inside a K or V tile).  K fragment c of half s:
   // token 32 s + r32, logical chunk 2 c + g (the swizzle repeats every 16
   // rows).  V^T fragment (dt, m, hh): lane i of a 16-lane group addresses
   // token 16 m + 8 hh + 4 g + i / 4, columns 32 dt + 16 dh + 4 (i % 4) .. + 3,
-  // and receives column i of the group's 16 for tokens j = 0..3.
-  // (Offsets of the other fragments differ from these by an XOR of bits the
-  // swizzles leave alone: chunk 2 c + g is (2 c) ^ g, d tile dt is chunk 4 dt
-  // ^ the tile's own, so they cost one instruction and no register.)
+  // and receives column i of the group's 16 for tokens j = 0..3.  (The other
+  // fragments' offsets differ by an XOR of bits the swizzles leave alone.)
   const int koff = 2 * (r32 * D + ((g ^ swz_k<D>(r32)) * 8));  // fragment c: koff ^ 32 c
   int voff[2];  // fragment (dt, hh): voff[hh] ^ 64 dt; the swizzle repeats every 8 rows
 #pragma unroll
@@ -176,8 +150,11 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
     voff[hh] = 2 * (t * D + (((c >> 3) ^ swz_v<D>(t)) << 3) + (c & 7));
   }
 
-  // DMA: row block i of this wave holds token rows (wave + NW i) TPI .. + TPI
-  // of a step, for K and for V; lane: row lane / CPR, physical chunk lane % CPR
+  const int n_it = (kve - kvb + kStep - 1) / kStep;
+  const int last_tok = kve - 1;
+  // ---- filling a slot, bf16 pool: row block i of this wave holds token rows
+  //      (wave + NW i) TPI .. + TPI of a step, for K and for V; lane: row
+  //      lane / CPR, physical chunk lane % CPR ----
   const size_t tok_bytes = (size_t)p.Hkv * D * 2;
   const char* kbase = reinterpret_cast<const char*>(p.kc + (size_t)h * D);
   const char* vbase = reinterpret_cast<const char*>(p.vc + (size_t)h * D);
@@ -194,13 +171,11 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
     d_v[i] = (pc ^ swz_v<D>(t)) * 16;
     d_lds[i] = t0 * D * 2;
   }
-  const int n_it = (kve - kvb + kStep - 1) / kStep;
-  const int last_tok = kve - 1;
+  // tokens past the item's end repeat its last one (masked out)
   auto issue = [&](int it, int slot) {
     const uint32_t sb = ring_lds + (uint32_t)slot * (2 * TILE * 2);
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
-      // tokens past the item's end repeat its last one (masked out)
       const int tok = min(kvb + it * kStep + d_t[i], last_tok);
       const int page = s_pages[min((tok >> p.log2P) - page0, kMaxItemPages - 1)];
       const size_t off = ((size_t)(uint32_t)page * P + (tok & (P - 1))) * tok_bytes;
@@ -208,8 +183,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
       dma16(sb + 2 * TILE + d_lds[i], vbase + off + d_v[i]);
     }
   };
-
-  // 8-bit pool: run i of this thread is codes 16 c8 .. + 15 of token row t8
+  // ---- 8-bit pool: run i of this thread is codes 16 c .. + 15 of token row t ----
   constexpr int NC = KV8 ? D / 16 / NW : 1;
   u32x4 k8[NC], v8[NC];
   uint32_t ke[NC], ve[NC];
@@ -267,40 +241,27 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
       sacc[s] = acc;
     }
   };
-  // online softmax over a step's 64 tokens (this lane: 32 of them)
-  auto softmax_of = [&](auto masked, int t0) {
-    constexpr bool MASKED = decltype(masked)::value;
-    float mx = kMaskVal;
+  auto mask = [&](int t0) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        if constexpr (MASKED) {
-          const int j = t0 + 32 * s + 8 * (i >> 2) + 4 * g + (i & 3);
-          if (j > lim || j >= kve) sacc[s][i] = kMaskVal;
-        }
-        mx = fmaxf(mx, sacc[s][i]);
+        const int j = t0 + 32 * s + 8 * (i >> 2) + 4 * g + (i & 3);
+        if (j > lim || j >= kve) sacc[s][i] = kMaskVal;
       }
+  };
+  auto row_max = [&]() {  // of the step's scores, as an exponent base
+    float mx = kMaskVal;
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sacc[s][i]);
     mx = max_xor32(mx);
-    mx = (MASKED && mx == kMaskVal) ? kMaskVal : mx * p.scale_log2;
-    const bool grow = mx > m_run + kLazyRescale;
-    if constexpr (KV8 || PART) {
-      // (always: around a branch the compiler keeps two copies of the
-      // accumulators, moves one to the other whichever way it goes, and spills)
-      const float mnew = grow ? mx : m_run;
-      const float alpha = __builtin_amdgcn_exp2f(m_run - mnew);
-      m_run = mnew;
-      l_run *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
-    } else if (__builtin_amdgcn_ballot_w64(grow)) {
-      const float mnew = grow ? mx : m_run;
-      const float alpha = __builtin_amdgcn_exp2f(m_run - mnew);
-      m_run = mnew;
-      l_run *= alpha;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) oacc[dt] *= alpha;
-    }
+    return mx == kMaskVal ? kMaskVal : mx * p.scale_log2;
+  };
+  auto full = [&](int t0) { return t0 + kStep - 1 <= w_lo && t0 + kStep <= kve; };
+  auto probs = [&](auto masked) {
+    constexpr bool MASKED = decltype(masked)::value;
     float ps = 0.f;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -320,11 +281,15 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
     }
     l_run += ps;
   };
+  int first = kvb;  // the step that sets the base (none in the second pass)
   auto softmax = [&](int t0) {
-    if (t0 + kStep - 1 <= w_lo && t0 + kStep <= kve)
-      softmax_of(std::false_type{}, t0);
+    const bool whole = full(t0);
+    if (!whole) mask(t0);
+    if (t0 == first) m_run = row_max();
+    if (whole)
+      probs(std::false_type{});
     else
-      softmax_of(std::true_type{}, t0);
+      probs(std::true_type{});
   };
   auto pv_mul = [&](int slot) {  // O^T += V^T P^T
     const char* Vt = reinterpret_cast<const char*>(&ring[slot][1][0]);
@@ -342,8 +307,8 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
       }
     }
   };
-  // A workgroup-wide phase boundary: every LDS read of this wave has
-  // returned, nothing moves across.
+  // A workgroup-wide phase boundary: every LDS access of this wave has
+  // completed, nothing moves across.
   auto phase = [&]() {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -352,104 +317,139 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
     asm volatile("" ::: "memory");
   };
 
-  if constexpr (PP) {
-    // Two wave groups half a step apart: a SIMD holds one wave of each, and
-    // while one runs its matrix phase (O += P V of step i - 1, S = K Q of
-    // step i) the other runs its softmax phase, so the matrix cores and the
-    // vector ALU work side by side.  Phase n of the workgroup: group 0 is in
-    // the matrix phase of step n / 2 (n even) or the softmax of n / 2 (odd),
-    // group 1 one phase behind.  Slot i % 4 is read in phases 2 i .. 2 i + 3
-    // (K by both groups, then V), so from phase 2 i + 4 on it takes step
-    // i + 4; a step's copies go out three phases ahead or more.
-    // (8-bit pool: step i + 4's conversion takes the place of its copies, a
-    // phase boundary makes it visible, and its successor's loads go out there)
-    const int grp = wave >> 2;
-    if constexpr (KV8) {
+  for (;;) {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) oacc[dt][i] = 0.f;
+    l_run = 0.f;
+    if constexpr (PP) {
+      // Two wave groups half a step apart: a SIMD holds one wave of each, and
+      // while one runs its matrix phase (O += P V of step i - 1, S = K Q of
+      // step i) the other runs its softmax phase, so the matrix cores and the
+      // vector ALU work side by side.  Phase n of the workgroup: group 0 is in
+      // the matrix phase of step n / 2 (n even) or the softmax of n / 2 (odd),
+      // group 1 one phase behind.  Slot i % 4 is read in phases 2 i .. 2 i + 3
+      // (K by both groups, then V), so from phase 2 i + 4 on it takes step
+      // i + 4; a step's copies go out three phases ahead or more (8-bit pool:
+      // its conversion is done there, one phase boundary before its first
+      // reader, and its successor's loads go out).
+      const int grp = wave >> 2;
+      if constexpr (KV8) {
+        fetch(0);
+        commit(0);
+        if (1 < n_it) {
+          fetch(1);
+          commit(1);
+        }
+        if (2 < n_it) fetch(2);
+      } else {
+        issue(0, 0);
+        if (1 < n_it) issue(1, 1);
+        wait_steps<NI, 1>(min(n_it - 1, 1));
+      }
+      phase();  // phase 0 begins: step 0 in LDS
+      if (grp == 1) {
+        if constexpr (KV8) {
+          if (2 < n_it) commit(2);
+          if (3 < n_it) fetch(3);
+        } else {
+          if (2 < n_it) issue(2, 2);
+          wait_steps<NI, 1>(min(max(n_it - 2, 0), 1));  // step 1 (if any) landed
+        }
+        phase();
+      }
+      bool had = false;  // the previous step's P is pending
+      for (int it = 0; it < n_it; ++it) {
+        const int t0 = kvb + it * kStep;
+        const bool vis = t0 <= w_hi;  // something visible to this wave's rows
+        if (had) pv_mul((it - 1) & 3);
+        if (vis) qk(it & 3);
+        had = vis;
+        if constexpr (!KV8) {
+          if (grp == 1) wait_steps<NI, 1>(min(max(n_it - 2 - it, 0), 1));
+        }
+        phase();
+        const int nx = it + 2 + grp;
+        if constexpr (KV8) {
+          if (nx < n_it) commit(nx & 3);
+          __builtin_amdgcn_sched_barrier(0);
+          if (nx + 1 < n_it) fetch(nx + 1);
+          __builtin_amdgcn_sched_barrier(0);
+        } else {
+          if (nx < n_it) issue(nx, nx & 3);
+        }
+        if (vis) softmax(t0);
+        if constexpr (!KV8) {
+          if (grp == 0) wait_steps<NI, 1>(min(max(n_it - 2 - it, 0), 1));
+        }
+        phase();
+      }
+      if (had) pv_mul((n_it - 1) & 3);
+      if (grp == 0) phase();  // group 1's last softmax phase
+    } else if constexpr (KV8) {
       fetch(0);
       commit(0);
-      if (1 < n_it) {
-        fetch(1);
-        commit(1);
+      if (1 < n_it) fetch(1);
+      for (int it = 0; it < n_it; ++it) {
+        phase();  // step `it` in LDS for every wave, the other slot free
+        if (it + 1 < n_it) commit((it + 1) & 1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (it + 2 < n_it) fetch(it + 2);
+        __builtin_amdgcn_sched_barrier(0);
+        const int t0 = kvb + it * kStep;
+        if (t0 > w_hi) continue;  // nothing visible to this wave's rows
+        qk(it & 1);
+        softmax(t0);
+        pv_mul(it & 1);
       }
-      if (2 < n_it) fetch(2);
     } else {
-      issue(0, 0);
-      if (1 < n_it) issue(1, 1);
-      wait_steps<NI, 1>(min(n_it - 1, 1));
-    }
-    phase();  // phase 0 begins: step 0 in LDS
-    if (grp == 1) {
-      if constexpr (KV8) {
-        if (2 < n_it) commit(2);
-        if (3 < n_it) fetch(3);
-      } else {
-        if (2 < n_it) issue(2, 2);
-        wait_steps<NI, 1>(min(max(n_it - 2, 0), 1));  // step 1 (if any) landed
-      }
-      phase();
-    }
-    bool had = false;  // the previous step's P is pending
-    for (int it = 0; it < n_it; ++it) {
-      const int t0 = kvb + it * kStep;
-      const bool vis = t0 <= w_hi;  // something visible to this wave's rows
-      if (had) pv_mul((it - 1) & 3);
-      if (vis) qk(it & 3);
-      had = vis;
-      if constexpr (!KV8) {
-        if (grp == 1) wait_steps<NI, 1>(min(max(n_it - 2 - it, 0), 1));
-      }
-      phase();
-      const int nx = it + 2 + grp;
-      if constexpr (KV8) {
-        if (nx < n_it) commit(nx & 3);
-        __builtin_amdgcn_sched_barrier(0);
-        if (nx + 1 < n_it) fetch(nx + 1);
-        __builtin_amdgcn_sched_barrier(0);
-      } else {
-        if (nx < n_it) issue(nx, nx & 3);
-      }
-      if (vis) softmax(t0);
-      if constexpr (!KV8) {
-        if (grp == 0) wait_steps<NI, 1>(min(max(n_it - 2 - it, 0), 1));
-      }
-      phase();
-    }
-    if (had) pv_mul((n_it - 1) & 3);
-    if (grp == 0) phase();  // group 1's last softmax phase
-  } else if constexpr (KV8) {
-    fetch(0);
-    commit(0);
-    if (1 < n_it) fetch(1);
-    for (int it = 0; it < n_it; ++it) {
-      phase();  // step `it` in LDS for every wave, the other slot free
-      if (it + 1 < n_it) commit((it + 1) & 1);
-      __builtin_amdgcn_sched_barrier(0);
-      if (it + 2 < n_it) fetch(it + 2);
-      __builtin_amdgcn_sched_barrier(0);
-      const int t0 = kvb + it * kStep;
-      if (t0 > w_hi) continue;
-      qk(it & 1);
-      softmax(t0);
-      pv_mul(it & 1);
-    }
-  } else {
 #pragma unroll
-    for (int it = 0; it < kNBuf - 1; ++it)
-      if (it < n_it) issue(it, it);
-    int slot = 0;
+      for (int it = 0; it < NBUF - 1; ++it)
+        if (it < n_it) issue(it, it);
+      int slot = 0;
+      for (int it = 0; it < n_it; ++it) {
+        // step `it` landed for this wave (the later issued steps stay in
+        // flight), and for every wave; slot (it - 1) is free
+        wait_steps<NI, NBUF - 2>(min(n_it - 1 - it, NBUF - 2));
+        phase();
+        const int cur = slot;
+        if (it + NBUF - 1 < n_it) issue(it + NBUF - 1, slot == 0 ? NBUF - 1 : slot - 1);
+        slot = slot + 1 == NBUF ? 0 : slot + 1;
+        const int t0 = kvb + it * kStep;
+        if (t0 > w_hi) continue;
+        qk(cur);
+        softmax(t0);
+        pv_mul(cur);
+      }
+    }
+    if (first < 0) break;
+    // did a row pass 2^60, or overflow?  (as integers: NaN counts too)
+    uint32_t top = __float_as_uint(l_run) >= 0x5d800000u ? 0x7f800000u : 0u;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(oacc[dt][i]) & 0x7fffffffu);
+    if (row_ok && top >= 0x7f800000u) s_redo = 1;
+    phase();
+    if (!__builtin_amdgcn_readfirstlane(s_redo)) break;
+    // a pass over K for the rows' maxima (no pipelining), then all once more
+    first = -1;
+    m_run = kMaskVal;
     for (int it = 0; it < n_it; ++it) {
-      // step `it` landed for this wave (the later issued steps stay in
-      // flight), and for every wave; slot (it - 1) is free
-      wait_steps<NI, kNBuf - 2>(min(n_it - 1 - it, kNBuf - 2));
+      if constexpr (KV8) {
+        fetch(it);
+        commit(0);
+      } else {
+        issue(it, 0);
+        wait_steps<NI, 0>(0);
+      }
       phase();
-      const int cur = slot;
-      if (it + kNBuf - 1 < n_it) issue(it + kNBuf - 1, slot == 0 ? kNBuf - 1 : slot - 1);
-      slot = slot + 1 == kNBuf ? 0 : slot + 1;
+      qk(0);
       const int t0 = kvb + it * kStep;
-      if (t0 > w_hi) continue;  // nothing visible to this wave's rows
-      qk(cur);
-      softmax(t0);
-      pv_mul(cur);
+      if (!full(t0)) mask(t0);
+      m_run = fmaxf(m_run, row_max());
+      phase();
     }
   }
 
@@ -470,36 +470,36 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void prefill_attn_kernel(
       prow[D] = m_run;
       prow[D + 1] = l;
     }
-    return;
+  } else {
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // l NaN stays NaN
+    bf16* orow = p.out + ((size_t)(qs + tau) * p.Hq + h * G + gam) * D + 4 * g;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int a = 0; a < 4; ++a) {
+        const floatx16 o = oacc[dt];
+        *reinterpret_cast<u32x2*>(orow + 32 * dt + 8 * a) =
+            u32x2{cvt_pk_bf16(o[4 * a] * inv, o[4 * a + 1] * inv),
+                  cvt_pk_bf16(o[4 * a + 2] * inv, o[4 * a + 3] * inv)};
+      }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  bf16* orow = p.out + ((size_t)(qs + tau) * p.Hq + h * G + gam) * D + 4 * g;
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const floatx16 o = oacc[dt];
-      *reinterpret_cast<u32x2*>(orow + 32 * dt + 8 * a) =
-          u32x2{cvt_pk_bf16(o[4 * a] * inv, o[4 * a + 1] * inv),
-                cvt_pk_bf16(o[4 * a + 2] * inv, o[4 * a + 3] * inv)};
-    }
 }
 
 template <bool KV8, bool PART>
-int32_t launch_prefill(int head_dim, int waves, int num_work, const AttnParams& prm,
-                       hipStream_t stream) {
+int32_t launch_tiles(int head_dim, int waves, int num_work, const AttnParams& prm,
+                     hipStream_t stream) {
   const dim3 grid(prm.Hkv, num_work), block(waves * 64);
   if (head_dim == 64 && waves == 4)
-    hipLaunchKernelGGL((prefill_attn_kernel<64, 4, KV8, PART>), grid, block, 0, stream, prm);
+    hipLaunchKernelGGL((attn_tile_kernel<64, 4, KV8, PART>), grid, block, 0, stream, prm);
   else if (head_dim == 128 && waves == 4)
-    hipLaunchKernelGGL((prefill_attn_kernel<128, 4, KV8, PART>), grid, block, 0, stream, prm);
+    hipLaunchKernelGGL((attn_tile_kernel<128, 4, KV8, PART>), grid, block, 0, stream, prm);
   else if (head_dim == 128 && waves == 8)
-    hipLaunchKernelGGL((prefill_attn_kernel<128, 8, KV8, PART>), grid, block, 0, stream, prm);
+    hipLaunchKernelGGL((attn_tile_kernel<128, 8, KV8, PART>), grid, block, 0, stream, prm);
   else {
-    set_error("prefill attention: head_dim %d, %d waves", head_dim, waves);
+    set_error("attention tiles: head_dim %d, %d waves", head_dim, waves);
     return NSG_ERR_ARG;
   }
-  return launch_status("prefill_attn_kernel");
+  return launch_status("attn_tile_kernel");
 }
 
 }  // namespace

@@ -14,7 +14,7 @@
 // prefix are read once per tile of up to 256 rows instead of once per request,
 // and a decode step's few rows per request fill MFMA tiles together.  Three
 // launches: the own parts and the prefix tiles leave partial rows (O, m, l; the
-// kernels of verify_attention.hip and prefill_attention.hpp, over shares of the
+// kernels of verify_attention.hip and prefill_tiles.hpp, over shares of the
 // KV range), the merge below joins a row's partials of both.
 #include <algorithm>
 #include <vector>
@@ -29,7 +29,6 @@ constexpr int kThreads = 256;
 constexpr int kBatch = 8;          // partial rows whose loads a merge thread has in flight
 constexpr int kAll = 0x3fffffff;   // causal limit of prefix tiles: everything is visible
 constexpr int kStep = 64;          // shares of a prefix are whole steps of this many tokens
-constexpr int kMinSteps = 4;       // ... at least this many
 
 struct MergeParams {
   const int* merge;
@@ -41,17 +40,24 @@ struct MergeParams {
 };
 
 // Merge item: [first query token, query tokens, first own item, own splits,
-// the group's first prefix item, its splits, its first query token, -].  A
-// thread owns 8 columns of a row and folds up to kBatch partials per memory
-// round trip.
-template <int D>
+// the group's first prefix item, its splits, its first query token, -].  A piece
+// is 8 columns of a row; its partials are folded in batches of kBatch, whose
+// loads are in flight together, by one lane, or (LANES = 4, few pieces: memory
+// round trips count) every fourth by each of the lanes l, l + 16, l + 32, l + 48 of
+// a wave, which then meet: 32 decode rows of 32 heads of 128 with 16 / 64 partials
+// 5.3 / 14 -> 4.3 / 10 us, but 576 rows with 8 partials 11.8 -> 24.
+template <int D, int LANES>
 __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(MergeParams p) {
   constexpr int PSTRIDE = D + 4;
   constexpr int CH = D / 8;
   const int* mw = p.merge + (size_t)blockIdx.x * NSG_ATTN_WORK_INTS;
   const int qs = mw[0], qn = mw[1], wi0 = mw[2], ns = mw[3], pw0 = mw[4], pns = mw[5];
-  const int item = (int)blockIdx.z * kThreads + (int)threadIdx.x;
-  if (item >= qn * p.G * CH) return;  // (a padding item has no query tokens)
+  const int lane = threadIdx.x & 63;
+  const int sub = LANES == 4 ? lane >> 4 : 0;
+  const int item = LANES == 4 ? ((int)blockIdx.z * (kThreads / 64) + (int)(threadIdx.x >> 6)) * 16 +
+                                    (lane & 15)
+                              : (int)blockIdx.z * kThreads + (int)threadIdx.x;
+  if (item >= qn * p.G * CH) return;  // whole pieces; a padding item has no query tokens
   const int h = blockIdx.y;
   const int row = item / CH;
   const int c0 = (item - row * CH) * 8;
@@ -68,11 +74,11 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(MergeParams p) {
   float M = kMaskVal, lsum = 0.f;
   float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const int n = ns + pns;
-  for (int s0 = 0; s0 < n; s0 += kBatch) {
+  for (int s0 = sub; s0 < n; s0 += LANES * kBatch) {
     floatx4 ml[kBatch], a[kBatch], b[kBatch];
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {  // past the last: re-reads it
-      const int s = min(s0 + j, n - 1);
+      const int s = min(s0 + LANES * j, n - 1);
       const float* r = s < ns ? own + s * own_step : pre + (s - ns) * pre_step;
       ml[j] = *reinterpret_cast<const floatx4*>(r + D);
       a[j] = *reinterpret_cast<const floatx4*>(r + c0);
@@ -80,7 +86,7 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(MergeParams p) {
     }
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
-      if (s0 + j >= n) break;
+      if (s0 + LANES * j >= n) break;
       const float Mn = fmaxf(M, ml[j][0]);
       const float sc = __builtin_amdgcn_exp2f(M - Mn);
       const float wt = __builtin_amdgcn_exp2f(ml[j][0] - Mn);
@@ -92,6 +98,13 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(MergeParams p) {
       }
       M = Mn;
     }
+  }
+  if constexpr (LANES == 4) {
+    const float sc = __builtin_amdgcn_exp2f(M - max_xor16_32(M));
+    lsum = sum_xor16_32(lsum * sc);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = sum_xor16_32(o[i] * sc);
+    if (sub) return;
   }
   const float inv = lsum > 0.f ? 1.f / lsum : (lsum == 0.f ? 0.f : lsum);
   bf16* orow = p.out + ((size_t)(qs + tau) * p.Hq + h * p.G + gam) * D + c0;
@@ -107,10 +120,26 @@ int prefix_rows(int64_t rows, int head_dim) {
   return rows <= 128 || head_dim == 64 ? 128 : 256;
 }
 
-// Prefix items aimed at: the workgroups that the GPU holds at once.
-int prefix_target(int rows, int head_dim, int num_cus, int num_kv_heads) {
-  const int per_cu = rows <= 64 ? 3 : rows == 256 ? 1 : head_dim == 64 ? 3 : 2;
-  return std::max(1, num_cus * per_cu / num_kv_heads);
+// Estimated time (us) of prefix tiles: a workgroup's start and 64-token step, the
+// steps a CU gets (workgroups sharing one take turns), the partial rows written
+// and read again, and the merge's round trips.  From 66 runs of the shapes below
+// over prefixes of 2048 - 16384 tokens, 1 - 64 steps per item; within 10 % where the
+// steps count.  (128 rows, 32 / 8 heads of 128, 4096 tokens: 32 / 16 / 8 / 4 items a
+// head 14.2 / 15.5 / 18.6 / 27.0 us; 2304 rows, 8192 tokens: 18 / 27 / 36 / 54 / 72
+// items 133 / 100 / 140 / 109 / 127, 36 being just over a round of workgroups.)
+struct TileFit {
+  double start, step;
+};
+TileFit tile_fit(int rows, int head_dim) {
+  if (rows <= 64) return head_dim == 64 ? TileFit{4.0, 0.37} : TileFit{5.0, 0.85};
+  if (head_dim == 64) return {5.5, 0.95};
+  return rows == 128 ? TileFit{8.0, 1.35} : TileFit{6.0, 2.25};
+}
+double tile_us(const TileFit& f, int64_t items, int64_t chunk, int shares, int rows, int head_dim,
+               int num_kv_heads, int num_cus) {
+  const int64_t wgs = items * num_kv_heads;
+  const double bytes = 2.0 * wgs * rows * (head_dim + 4) * 4;
+  return f.start + f.step * chunk * ((wgs + num_cus - 1) / num_cus) + bytes / 5.0e6 + 0.12 * shares;
 }
 
 struct Sizes {
@@ -130,17 +159,26 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
                 groups[num_groups]);
   NSG_CHECK_ARG(pkv[0] == 0, "prefix_kv_indptr must start at 0");
   if (num_cus <= 0) num_cus = 256;
-  // ---- the own parts: an attention plan whose items all leave partials ----
+  NSG_CHECK_ARG(Hkv > 0 && Hq > 0 && Hq % Hkv == 0,
+                "num_qo_heads %d must be a positive multiple of num_kv_heads %d", Hq, Hkv);
+  const int G = Hq / Hkv;
+  // ---- the own parts: an attention plan whose items all leave partials.  The
+  //      merge is there anyway, so several KV groups per workgroup (whole CUs
+  //      per tile of 16 rows) only while every tile has a CU ----
+  int64_t tiles16 = 0;
+  const int t16 = std::max(1, 16 / G);
+  if (sz.fixed)
+    tiles16 = (int64_t)sz.max_batch * ((sz.max_q_len + t16 - 1) / t16);
+  else
+    for (int b = 0; b < batch; ++b) tiles16 += (qo[b + 1] - qo[b] + t16 - 1) / t16;
+  const int regime = tiles16 * Hkv <= num_cus ? 1 : 0;
   std::vector<int32_t> own(1024 * NSG_ATTN_WORK_INTS);
   nsg_attn_plan_t op{};
   for (;;) {
     const int32_t cap = (int32_t)(own.size() / NSG_ATTN_WORK_INTS);
-    const int32_t rc =
-        sz.fixed ? nsg_attn_plan_fixed(qo, kvp, last, batch, Hq, Hkv, head_dim, page_size, causal,
-                                       num_cus, sz.max_q_len, sz.max_kv_len, sz.max_work,
-                                       sz.max_merge, own.data(), cap, &op)
-                 : nsg_attn_plan(qo, kvp, last, batch, Hq, Hkv, head_dim, page_size, causal,
-                                 num_cus, own.data(), cap, &op);
+    const int32_t rc = plan_attn(qo, kvp, last, batch, Hq, Hkv, head_dim, page_size, causal,
+                                 num_cus, own.data(), cap, sz.fixed ? sz.max_work : -1,
+                                 sz.max_merge, sz.max_q_len, sz.max_kv_len, regime, &op);
     if (rc == NSG_OK) break;
     // (a fixed list that is too small stays so whatever the buffer)
     const bool grow = rc == NSG_ERR_WORKSPACE &&
@@ -148,7 +186,6 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
     if (!grow) return rc;
     own.resize(own.size() * 4);
   }
-  const int G = Hq / Hkv;
   // ---- the prefix tiles ----
   int64_t most = 0;
   for (int g = 0; g < num_groups; ++g) {
@@ -168,13 +205,32 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
     return np ? (np - 1) * page_size + plast[g] : 0;
   };
   auto tiles_of = [&](int g) { return (qo[groups[g + 1]] - qo[groups[g]] + T - 1) / T; };
-  int64_t total = 0;
+  // Steps per item: of the shares that the longest prefix can be cut into, the
+  // number with the least estimated time (an item's page ids must fit the
+  // kernels' list, the items a fixed list)
+  int64_t longest = 0;
   for (int g = 0; g < num_groups; ++g)
-    total += (int64_t)tiles_of(g) * ((prefix_len(g) + kStep - 1) / kStep);
-  const int target = prefix_target(rows, head_dim, num_cus, Hkv);
-  int64_t chunk = std::max<int64_t>(kMinSteps, (total + target - 1) / target);
-  // an item's page ids must fit the kernels' list
-  chunk = std::min(chunk, std::max<int64_t>(1, (int64_t)(kMaxItemPages - 2) * page_size / kStep));
+    if (tiles_of(g)) longest = std::max<int64_t>(longest, (prefix_len(g) + kStep - 1) / kStep);
+  const int64_t by_pages =
+      std::max<int64_t>(1, (int64_t)(kMaxItemPages - 2) * page_size / kStep);
+  const int64_t fewest = (longest + by_pages - 1) / by_pages;
+  const TileFit fit = tile_fit(rows, head_dim);
+  int64_t chunk = 1;
+  double best = -1;
+  for (int64_t n = std::max<int64_t>(1, fewest); n <= std::max(fewest, std::min<int64_t>(longest, 64));
+       ++n) {
+    const int64_t c = (longest + n - 1) / n;
+    int64_t items = 0;
+    for (int g = 0; g < num_groups; ++g)
+      items += tiles_of(g) * (((prefix_len(g) + kStep - 1) / kStep + c - 1) / c);
+    if (sz.fixed && items > sz.max_prefix_work && best >= 0) break;
+    const double us = tile_us(fit, items, c, (int)n, (int)std::min<int64_t>(rows, most), head_dim,
+                              Hkv, num_cus);
+    if (best < 0 || us < best) {
+      best = us;
+      chunk = c;
+    }
+  }
   std::vector<int32_t> pre;
   std::vector<int> first(num_groups), splits(num_groups);
   for (int g = 0; g < num_groups; ++g) {
@@ -217,6 +273,9 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
   plan->num_merge = sz.fixed ? sz.max_merge : n_merge;
   plan->prefix_rows = rows;
   plan->prefix_tile_tokens = T;
+  const int64_t q_rows = sz.fixed ? (int64_t)sz.max_batch * sz.max_q_len : qo[batch];
+  plan->merge_lanes = q_rows * Hq * (head_dim / 8) <= 65536 ? 4 : 1;
+  plan->prefix_kv_groups = rows <= 64 && page_size >= 16 ? (head_dim == 64 ? 4 : 2) : 1;
   const int64_t row_bytes = (int64_t)Hkv * (head_dim + 4) * 4;
   plan->prefix_partials = kHeader + (int64_t)op.num_work * op.row_tiles * 16 * row_bytes;
   plan->workspace_bytes = plan->prefix_partials + (int64_t)plan->num_prefix_work * rows * row_bytes;
@@ -299,7 +358,7 @@ extern "C" int32_t nsg_prefix_attn_fixed_capacity(int32_t batch, int32_t max_q_l
   const int64_t by_pages =
       std::max<int64_t>(1, (int64_t)(kMaxItemPages - 2) * page_size / kStep);
   const int64_t forced = tiles * ((steps + by_pages - 1) / by_pages);
-  const int64_t n = std::max(forced, prefix_target(rows, head_dim, num_cus, num_kv_heads) + tiles);
+  const int64_t n = std::max<int64_t>(forced, 2 * num_cus / num_kv_heads + tiles);
   NSG_CHECK_ARG(n <= 1 << 24, "too many prefix items (%lld)", (long long)n);
   *max_prefix_work = (int32_t)n;
   *max_merge = *max_work;  // every query tile of the own parts meets its prefix
@@ -317,6 +376,11 @@ extern "C" int32_t nsg_prefix_attn_plan_fixed(
     int32_t work_capacity, nsg_prefix_attn_plan_t* plan) {
   NSG_CHECK_ARG(max_prefix_work >= 0, "max_prefix_work %d", max_prefix_work);
   NSG_CHECK_ARG(batch <= max_batch, "batch %d exceeds the fixed plan's %d", batch, max_batch);
+  NSG_CHECK_ARG(max_q_len >= 1 && max_work >= 1 && max_merge >= 1,
+                "max_q_len %d, max_work %d, max_merge %d", max_q_len, max_work, max_merge);
+  NSG_CHECK_ARG(page_size > 0 && max_kv_len <= (kMaxItemPages - 2) * (int64_t)page_size,
+                "max_kv_len %d exceeds one work item's page list (%lld tokens)", max_kv_len,
+                (kMaxItemPages - 2) * (long long)page_size);
   return guarded([&] {
     return plan_impl(qo_indptr_h, group_indptr_h, num_groups, prefix_kv_indptr_h,
                      prefix_kv_last_page_len_h, kv_indptr_h, kv_last_page_len_h, batch,
@@ -355,9 +419,10 @@ extern "C" int32_t nsg_prefix_attn_run(const nsg_prefix_attn_plan_t* plan, const
     set_error("head_dim %d not supported", own.head_dim);
     return NSG_ERR_UNSUPPORTED;
   }
-  NSG_CHECK_ARG(own.kv_groups == 1 || page_size >= 16,
+  NSG_CHECK_ARG((own.kv_groups == 1 && plan->prefix_kv_groups == 1) || page_size >= 16,
                 "page_size %d: the plan's %d KV groups need pages of 16+ tokens (plan and run "
-                "with the same page size)", page_size, own.kv_groups);
+                "with the same page size)", page_size, std::max(own.kv_groups,
+                                                               plan->prefix_kv_groups));
   if (workspace_bytes < plan->workspace_bytes) {
     set_error("workspace has %lld bytes, plan needs %lld", (long long)workspace_bytes,
               (long long)plan->workspace_bytes);
@@ -384,8 +449,8 @@ extern "C" int32_t nsg_prefix_attn_run(const nsg_prefix_attn_plan_t* plan, const
   hipStream_t s = static_cast<hipStream_t>(stream);
   auto launch = [&](const nsg_attn_plan_t& pl) {
     if (pl.row_tiles >= 8)
-      return (fp8 ? launch_prefill_part_fp8 : launch_prefill_part)(pl.head_dim, pl.row_tiles / 2,
-                                                                   pl.num_work, prm, s);
+      return fp8 ? launch_tiles_part_fp8(pl.head_dim, pl.row_tiles / 2, pl.num_work, prm, s)
+                 : launch_tiles_part(pl.head_dim, pl.row_tiles / 2, pl.num_work, prm, s);
     return (fp8 ? launch_verify_attn_fp8 : launch_verify_attn)(&pl, prm, s);
   };
   // own parts
@@ -400,7 +465,7 @@ extern "C" int32_t nsg_prefix_attn_run(const nsg_prefix_attn_plan_t* plan, const
     nsg_attn_plan_t pp = own;
     pp.num_work = plan->num_prefix_work;
     pp.row_tiles = plan->prefix_rows / 16;
-    pp.kv_groups = 1;
+    pp.kv_groups = plan->prefix_kv_groups;
     prm.work = work_p;
     prm.num_work = pp.num_work;
     prm.kv_indices = prefix_kv_indices;
@@ -418,12 +483,19 @@ extern "C" int32_t nsg_prefix_attn_run(const nsg_prefix_attn_plan_t* plan, const
   m.Hq = prm.Hq;
   m.Hkv = prm.Hkv;
   m.G = prm.G;
+  const int pieces = kThreads / plan->merge_lanes;  // a workgroup's
   const unsigned slices =
-      (unsigned)((own.q_tile_tokens * prm.G * (own.head_dim / 8) + kThreads - 1) / kThreads);
+      (unsigned)((own.q_tile_tokens * prm.G * (own.head_dim / 8) + pieces - 1) / pieces);
   const dim3 grid(plan->num_merge, prm.Hkv, slices);
-  if (own.head_dim == 64)
-    hipLaunchKernelGGL(prefix_merge_kernel<64>, grid, dim3(kThreads), 0, s, m);
+  const dim3 block(kThreads);
+  const bool four = plan->merge_lanes == 4;
+  if (own.head_dim == 64 && four)
+    hipLaunchKernelGGL((prefix_merge_kernel<64, 4>), grid, block, 0, s, m);
+  else if (own.head_dim == 64)
+    hipLaunchKernelGGL((prefix_merge_kernel<64, 1>), grid, block, 0, s, m);
+  else if (four)
+    hipLaunchKernelGGL((prefix_merge_kernel<128, 4>), grid, block, 0, s, m);
   else
-    hipLaunchKernelGGL(prefix_merge_kernel<128>, grid, dim3(kThreads), 0, s, m);
+    hipLaunchKernelGGL((prefix_merge_kernel<128, 1>), grid, block, 0, s, m);
   return launch_status("prefix_merge_kernel");
 }

@@ -999,7 +999,8 @@ int max_splits_planned(const std::vector<int>& split_counts) {
   return mx;
 }
 
-// Shared planner.  fixed_work < 0: the work list holds exactly the items the
+// Shared planner.  regime: 1 several KV groups per workgroup (where the pages
+// allow), 0 one, -1 by the rule below.  fixed_work < 0: the work list holds exactly the items the
 // plan needs.  fixed_work >= 0: it holds exactly fixed_work work items (the
 // tail padded with empty items, query tokens 0) followed by fixed_merge merge
 // items (padded with split count 0), so that nsg_attn_run launches the same
@@ -1009,7 +1010,7 @@ int32_t plan_impl(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
                   int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int32_t causal,
                   int32_t num_cus, int32_t* work_h, int32_t work_capacity, int32_t fixed_work,
                   int32_t fixed_merge, int32_t fixed_q_len, int32_t fixed_kv_len,
-                  nsg_attn_plan_t* plan) {
+                  int32_t regime, nsg_attn_plan_t* plan) {
   NSG_CHECK_ARG(plan && qo_indptr_h && kv_indptr_h && kv_last_page_len_h, "null argument");
   NSG_CHECK_ARG(batch >= 0, "batch %d < 0", batch);
   NSG_CHECK_ARG(num_kv_heads > 0 && num_qo_heads > 0 && num_qo_heads % num_kv_heads == 0,
@@ -1089,13 +1090,14 @@ int32_t plan_impl(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
                         num_cus);
   const bool compare = pre.rows && pre.wgs < 2ll * num_cus;
   if (fixed_work >= 0) {
-    latency = page_size >= kMinGroupPage && fixed_kv_len > 0;
+    latency = page_size >= kMinGroupPage && fixed_kv_len > 0 && regime != 0;
     T = q_tile_tokens(G, max_ql, latency);
     if (int32_t rc = make_groups(T)) return rc;
   } else if (!pre.rows || compare) {
     T = q_tile_tokens(G, max_ql, false);
     if (int32_t rc = make_groups(T)) return rc;
-    latency = page_size >= kMinGroupPage && (total_it + t1 - 1) / t1 <= kMinSplitSteps;
+    latency = page_size >= kMinGroupPage &&
+              (regime < 0 ? (total_it + t1 - 1) / t1 <= kMinSplitSteps : regime > 0);
     if (latency && q_tile_tokens(G, max_ql, true) != T) {
       T = q_tile_tokens(G, max_ql, true);
       if (int32_t rc = make_groups(T)) return rc;
@@ -1279,6 +1281,18 @@ int32_t plan_impl(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
 }
 
 }  // namespace
+
+int32_t plan_attn(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
+                  const int32_t* kv_last_page_len_h, int32_t batch, int32_t num_qo_heads,
+                  int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int32_t causal,
+                  int32_t num_cus, int32_t* work_h, int32_t work_capacity, int32_t fixed_work,
+                  int32_t fixed_merge, int32_t fixed_q_len, int32_t fixed_kv_len, int32_t regime,
+                  nsg_attn_plan_t* plan) {
+  return plan_impl(qo_indptr_h, kv_indptr_h, kv_last_page_len_h, batch, num_qo_heads,
+                   num_kv_heads, head_dim, page_size, causal, num_cus, work_h, work_capacity,
+                   fixed_work, fixed_merge, fixed_q_len, fixed_kv_len, regime, plan);
+}
+
 }  // namespace nsg
 
 extern "C" int32_t nsg_attn_plan(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
@@ -1288,7 +1302,7 @@ extern "C" int32_t nsg_attn_plan(const int32_t* qo_indptr_h, const int32_t* kv_i
                                  int32_t* work_h, int32_t work_capacity, nsg_attn_plan_t* plan) {
   return plan_impl(qo_indptr_h, kv_indptr_h, kv_last_page_len_h, batch, num_qo_heads,
                    num_kv_heads, head_dim, page_size, causal, num_cus, work_h, work_capacity,
-                   -1, 0, 0, 0, plan);
+                   -1, 0, 0, 0, -1, plan);
 }
 
 extern "C" int32_t nsg_attn_fixed_capacity(int32_t batch, int32_t max_q_len,
@@ -1322,7 +1336,7 @@ extern "C" int32_t nsg_attn_plan_fixed(const int32_t* qo_indptr_h, const int32_t
                 (kMaxItemPages - 2) * page_size);
   return plan_impl(qo_indptr_h, kv_indptr_h, kv_last_page_len_h, batch, num_qo_heads,
                    num_kv_heads, head_dim, page_size, causal, num_cus, work_h, work_capacity,
-                   max_work, max_merge, max_q_len, max_kv_len, plan);
+                   max_work, max_merge, max_q_len, max_kv_len, -1, plan);
 }
 
 extern "C" int32_t nsg_attn_run(const nsg_attn_plan_t* plan, const int32_t* work_d,

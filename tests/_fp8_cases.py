@@ -85,6 +85,13 @@ def attention(q, spans, q_lens, causal=True, scale=None):
     return out, bound
 
 
+def ramp(rng, n, Hkv, D, slope):
+    """K rows that every positive query scores slope * (j / n) higher or lower
+    with position j: n rows of one direction, exact in e4m3 with their scale."""
+    a = np.round(slope * np.arange(n) / n * 4) / 4
+    return bf16(np.repeat(a[:, None, None], Hkv, 1) * np.ones(D))
+
+
 def check(got, want, bound):
     """got (bf16 tensor) within bound of want; where want is NaN got is."""
     g = got.double().cpu().numpy()

@@ -134,6 +134,29 @@ def test_nan_rows_reach_only_who_sees_them(q_lens, kv_lens, what):
         t0 += n
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,q_lens,kv_lens", [
+    (14, 2, 64, [1, 5, 3], [300, 640, 70]), (32, 8, 128, [9, 9], [4000, 5001]),
+    (8, 1, 128, [1], [9000]), (32, 8, 128, [1000, 900, 800], [1000, 1500, 800]),
+    (14, 2, 64, [500] * 20, [500] * 20), (48, 1, 64, [1, 2], [700, 800])])
+@pytest.mark.parametrize("slope", [14.0, -14.0])
+def test_scores_that_leave_the_first_steps_maximum_far_behind(Hq, Hkv, D, q_lens, kv_lens, slope):
+    """Scores that rise (or fall) by several hundred along a context: far past
+    2^127 times the first step's probabilities."""
+    from oracle import kv_fp8
+    c = _case(16, q_lens, kv_lens, Hq, Hkv, D, 16)
+    kc, vc, sc = (x.copy() for x in c["pool"][:3])
+    rng = np.random.default_rng(0)
+    for tab, n in zip(c["tabs"], kv_lens):
+        codes, e = kv_fp8.quantise(fc.ramp(rng, n, Hkv, D, slope), False)
+        for j in range(n):
+            kc[tab[j // 16], j % 16] = codes[j]
+            sc[tab[j // 16], :, 0, j % 16] = e[j]
+    c["pool"] = (kc, vc, sc, *fc.values(kc, vc, sc))
+    c["q"] = fc.bf16(np.abs(c["q"]) + 3)
+    got, _ = _run(c)
+    fc.check(got, *_want(c))
+
+
 def test_rows_behind_the_last_token_are_not_read():
     """Slots past a request's length, on its own last page and on others, may
     hold anything: NaN codes and NaN scales change nothing."""
@@ -216,13 +239,14 @@ def test_graph_plans_replay_over_growing_contexts(max_kv_len):
         fc.check(out, *fc.attention(x, spans, [q] * B))
 
 
-def test_equals_the_bf16_pool_of_the_same_values():
-    """Prefill tiles convert into the bf16 kernel's own: the same bits as that
-    kernel over a bf16 pool of the same values."""
-    c = _case(15, [1024, 1000], [1024, 1800], 32, 8, 128, 16)
-    got, w = _run(c)
-    assert w.plan_info.row_tiles == 16
-    k, v = (torch.from_numpy(x).cuda().bfloat16() for x in c["pool"][3:])
-    w2 = _wrapper()
-    w2.plan(c["qo"], c["ptr"], c["idx"], c["last"], *c["dims"])
-    assert torch.equal(got, w2.run(torch.from_numpy(c["q"]).cuda().bfloat16(), (k, v)))
+def test_agrees_with_the_bf16_pool_of_the_same_values():
+    """The bf16 kernels over a bf16 pool of the same values: both within their
+    bound of the same reference."""
+    for q_lens, kv_lens in (([1024, 1000], [1024, 1800]), ([5, 9, 1], [300, 2000, 64])):
+        c = _case(15, q_lens, kv_lens, 32, 8, 128, 16)
+        want, bound = _want(c)
+        fc.check(_run(c)[0], want, bound)
+        k, v = (torch.from_numpy(x).cuda().bfloat16() for x in c["pool"][3:])
+        w = _wrapper()
+        w.plan(c["qo"], c["ptr"], c["idx"], c["last"], *c["dims"])
+        fc.check(w.run(torch.from_numpy(c["q"]).cuda().bfloat16(), (k, v)), want, bound)

@@ -120,6 +120,39 @@ def test_prompts_long_own_parts_and_a_long_prefix(fp8):
           fp8)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("heads,n,q", [((14, 2, 64), 3, 1), ((14, 2, 64), 33, 5),
+                                       ((32, 8, 128), 3, 1), ((32, 8, 128), 25, 1),
+                                       ((32, 8, 128), 30, 9)])
+def test_scores_that_leave_the_first_steps_maximum_far_behind(heads, n, q, fp8):
+    """Scores that rise by several hundred along the prefix, past 2^127 times
+    its first step's probabilities, and fall along the own parts."""
+    from oracle import kv_fp8
+    Hq, Hkv, D = heads
+    rng = np.random.default_rng(9)
+    P, pages = 16, 900
+    c = dict(q=[q] * n, kv=[int(q + x) for x in rng.integers(0, 200, n)], groups=[0, n],
+             prefix=[1500])
+    ptabs, tabs = _tables(rng, c, P, pages)
+    k, v = (fc.rows(rng, pages, P, Hkv, D) for _ in range(2))
+    for tab, m, slope in [(ptabs[0], 1500, 14.0)] + [(t, m, -9.0) for t, m in zip(tabs, c["kv"])]:
+        r = fc.ramp(rng, m, Hkv, D, slope)
+        for j in range(m):
+            k[tab[j // P], j % P] = r[j]
+    if fp8:
+        (kc, ke), (vc, ve) = kv_fp8.quantise(k, False), kv_fp8.quantise(v, True)
+        scale = np.ascontiguousarray(np.stack([ke, ve], 2).transpose(0, 3, 2, 1))
+        k, v = fc.values(kc, vc, scale)
+        *caches, sc = fc.on_gpu(kc, vc, scale)
+    else:
+        caches, sc = [torch.from_numpy(x).cuda().bfloat16() for x in (k, v)], None
+    x = fc.bf16(np.abs(rng.standard_normal((n * q, Hq, D))) + 3)
+    w = _wrapper()
+    _plan(w, c, ptabs, tabs, heads, P, fp8)
+    got = w.run(torch.from_numpy(x).cuda().bfloat16(), caches, kv_scale=sc)
+    fc.check(got, *_want(x, c, ptabs, tabs, k, v))
+
+
 def test_not_causal_and_own_scale():
     _case(3, dict(q=[5, 3], kv=[2, 100], groups=[0, 2], prefix=[50]), (14, 2, 64), 16, False,
           causal=False, sm_scale=0.4)
