@@ -173,6 +173,8 @@ typedef struct {
   int32_t prefix_tile_tokens; /* query tokens of a prefix tile                */
   int32_t prefix_kv_groups;   /* KV groups per prefix workgroup               */
   int32_t merge_lanes;        /* lanes that share a row's partials            */
+  int32_t one_launch;         /* prefix and own items in one list and launch  */
+  int32_t own_rows;           /* partial rows per own item                    */
   int64_t prefix_partials;    /* byte offset of the prefix partials           */
   int64_t workspace_bytes;    /* device workspace nsg_prefix_attn_run needs   */
 } nsg_prefix_attn_plan_t;
@@ -211,15 +213,16 @@ int32_t nsg_prefix_attn_plan_fixed(
     int32_t work_capacity, nsg_prefix_attn_plan_t* plan);
 
 /* Runs one layer over the bf16 pool (kv_scale NULL) or the 8-bit one.  work_d:
- * device copy of the planner's list; the workspace starts with the same
- * error-flag word as nsg_attn_run's (nsg_attn_check_flags).  q, out and the
- * caches must be 16-byte aligned. */
+ * device copy of the planner's list; kv_indices: the prefixes' page ids
+ * (prefix_kv_indptr[num_groups] of them), then the batch's; the workspace
+ * starts with the same error-flag word as nsg_attn_run's (nsg_attn_check_flags).
+ * q, out and the caches must be 16-byte aligned. */
 int32_t nsg_prefix_attn_run(const nsg_prefix_attn_plan_t* plan, const int32_t* work_d,
                             const void* q, const void* k_cache, const void* v_cache,
-                            const void* kv_scale, void* out, const int32_t* prefix_kv_indices,
-                            const int32_t* kv_indices, int32_t page_size, int32_t num_pages,
-                            float sm_scale, int32_t causal, void* workspace,
-                            int64_t workspace_bytes, nsg_stream_t stream);
+                            const void* kv_scale, void* out, const int32_t* kv_indices,
+                            int32_t page_size, int32_t num_pages, float sm_scale,
+                            int32_t causal, void* workspace, int64_t workspace_bytes,
+                            nsg_stream_t stream);
 
 /* Copies the workspace's error flags (bit 0: page id out of range) to
  * *flags_h after synchronising the stream, and clears them. */

@@ -33,6 +33,7 @@ class PrefixAttnPlan(C.Structure):
     _fields_ = [
         ("own", AttnPlan), ("num_prefix_work", i32), ("num_merge", i32), ("prefix_rows", i32),
         ("prefix_tile_tokens", i32), ("prefix_kv_groups", i32), ("merge_lanes", i32),
+        ("one_launch", i32), ("own_rows", i32),
         ("prefix_partials", i64), ("workspace_bytes", i64),
     ]
 
@@ -85,8 +86,8 @@ SIGNATURES = {
     "nsg_prefix_attn_plan_fixed": (i32, [vp, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, i32,
                                          i32, i32, i32, i32, i32, i32, i32, i32, vp, i32,
                                          C.POINTER(PrefixAttnPlan)]),
-    "nsg_prefix_attn_run": (i32, [C.POINTER(PrefixAttnPlan), vp, vp, vp, vp, vp, vp, vp, vp, i32,
-                                  i32, f32, i32, vp, i64, vp]),
+    "nsg_prefix_attn_run": (i32, [C.POINTER(PrefixAttnPlan), vp, vp, vp, vp, vp, vp, vp, i32, i32,
+                                  f32, i32, vp, i64, vp]),
     "nsg_attn_check_flags": (i32, [vp, C.POINTER(i32), vp]),
     "nsg_spec_accept_check_flags": (i32, [vp, i64, C.POINTER(i32), vp]),
     "nsg_spec_accept_greedy_tokens": (i32, [vp, vp, i64, i64, i32, i32, i32, vp, vp, vp, i32,

@@ -12,10 +12,11 @@
 // The prefix is attended to once per group: its query tiles run over the
 // group's packed query tokens as if they were one request, so K and V of the
 // prefix are read once per tile of up to 256 rows instead of once per request,
-// and a decode step's few rows per request fill MFMA tiles together.  Three
-// launches: the own parts and the prefix tiles leave partial rows (O, m, l; the
-// kernels of verify_attention.hip and prefill_tiles.hpp, over shares of the
-// KV range), the merge below joins a row's partials of both.
+// and a decode step's few rows per request fill MFMA tiles together.  The own
+// parts and the prefix tiles leave partial rows (O, m, l; the kernels of
+// verify_attention.hip, verify_attention_fp8.hip and prefill_tiles.hpp, over
+// shares of the KV range), in one launch where groups have few rows, else in
+// two; the merge below joins a row's partials of both.
 #include <algorithm>
 #include <vector>
 
@@ -120,13 +121,11 @@ int prefix_rows(int64_t rows, int head_dim) {
   return rows <= 128 || head_dim == 64 ? 128 : 256;
 }
 
-// Estimated time (us) of prefix tiles: a workgroup's start and 64-token step, the
-// steps a CU gets (workgroups sharing one take turns), the partial rows written
-// and read again, and the merge's round trips.  From 66 runs of the shapes below
-// over prefixes of 2048 - 16384 tokens, 1 - 64 steps per item; within 10 % where the
-// steps count.  (128 rows, 32 / 8 heads of 128, 4096 tokens: 32 / 16 / 8 / 4 items a
-// head 14.2 / 15.5 / 18.6 / 27.0 us; 2304 rows, 8192 tokens: 18 / 27 / 36 / 54 / 72
-// items 133 / 100 / 140 / 109 / 127, 36 being just over a round of workgroups.)
+// Estimated times (us).  A kernel: a workgroup's start and 64-token step.  From 66
+// runs of prefixes of 2048 - 16384 tokens at 1 - 64 steps per item; within 10 % where
+// the steps count.  (128 rows, 32 / 8 heads of 128, 4096 tokens: 32 / 16 / 8 / 4 items
+// a head 14.2 / 15.5 / 18.6 / 27.0; 2304 rows, 8192 tokens: 18 / 27 / 36 / 54 / 72 items
+// 133 / 100 / 140 / 109 / 127, 36 being just over a round of workgroups.)
 struct TileFit {
   double start, step;
 };
@@ -135,12 +134,23 @@ TileFit tile_fit(int rows, int head_dim) {
   if (head_dim == 64) return {5.5, 0.95};
   return rows == 128 ? TileFit{8.0, 1.35} : TileFit{6.0, 2.25};
 }
-double tile_us(const TileFit& f, int64_t items, int64_t chunk, int shares, int rows, int head_dim,
-               int num_kv_heads, int num_cus) {
-  const int64_t wgs = items * num_kv_heads;
-  const double bytes = 2.0 * wgs * rows * (head_dim + 4) * 4;
-  return f.start + f.step * chunk * ((wgs + num_cus - 1) / num_cus) + bytes / 5.0e6 + 0.12 * shares;
+// The partial rows of a prefix written and read again, and the merge's round trips.
+double partials_us(int64_t wgs, int rows, int head_dim, int shares) {
+  return 2.0 * wgs * rows * (head_dim + 4) * 4 / 5.0e6 + 0.12 * shares;
 }
+// One launch of items of at most `longest` steps, `steps` over all workgroups, where a
+// CU's workgroups take turns: a start per round, and the steps over the CUs with
+// a third of the longest item left over at the end (in whole items where all
+// are alike).
+double launch_us(const TileFit& f, int64_t wgs, double steps, int64_t longest, bool alike,
+                 int num_cus) {
+  const int64_t rounds = (wgs + num_cus - 1) / num_cus;
+  return alike ? f.start + f.step * longest * rounds
+               : f.start * rounds +
+                     f.step * std::max((double)longest, steps / num_cus + 0.3 * longest);
+}
+constexpr double kLaunchGap = 1.5;
+constexpr int kFixedJointRows = 512;  // fixed plans: one launch up to so many rows
 
 struct Sizes {
   bool fixed;
@@ -162,16 +172,31 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
   NSG_CHECK_ARG(Hkv > 0 && Hq > 0 && Hq % Hkv == 0,
                 "num_qo_heads %d must be a positive multiple of num_kv_heads %d", Hq, Hkv);
   const int G = Hq / Hkv;
+  NSG_CHECK_ARG(page_size > 0, "page_size %d must be a power of two", page_size);
+  int64_t most = 0;  // rows of the largest group
+  for (int g = 0; g < num_groups; ++g) {
+    NSG_CHECK_ARG(groups[g] <= groups[g + 1] && groups[g + 1] <= batch,
+                  "group %d: decreasing group_indptr", g);
+    const int np = pkv[g + 1] - pkv[g];
+    NSG_CHECK_ARG(np >= 0, "group %d: decreasing prefix_kv_indptr", g);
+    NSG_CHECK_ARG(np == 0 || (plast[g] >= 1 && plast[g] <= page_size),
+                  "group %d: prefix last_page_len %d outside [1, %d]", g, plast[g], page_size);
+    NSG_CHECK_ARG(np <= kAll / page_size, "group %d: prefix of %d pages", g, np);
+    most = std::max<int64_t>(most, (int64_t)(qo[groups[g + 1]] - qo[groups[g]]) * G);
+  }
+  if (sz.fixed) most = (int64_t)sz.max_batch * sz.max_q_len * G;
   // ---- the own parts: an attention plan whose items all leave partials.  The
-  //      merge is there anyway, so several KV groups per workgroup (whole CUs
-  //      per tile of 16 rows) only while every tile has a CU ----
+  //      merge is there anyway, so several KV groups per workgroup (a whole CU
+  //      per tile of 16 rows) only for up to two rounds of tiles (64 decode
+  //      rows of 32 / 8 heads of 128 behind 300 / 4000 tokens 29 / 41 -> 21 / 32 us;
+  //      four rounds, 320 rows behind 4000: 61 -> 83) ----
   int64_t tiles16 = 0;
   const int t16 = std::max(1, 16 / G);
   if (sz.fixed)
     tiles16 = (int64_t)sz.max_batch * ((sz.max_q_len + t16 - 1) / t16);
   else
     for (int b = 0; b < batch; ++b) tiles16 += (qo[b + 1] - qo[b] + t16 - 1) / t16;
-  const int regime = tiles16 * Hkv <= num_cus ? 1 : 0;
+  const int regime = tiles16 * Hkv <= 2 * num_cus ? 1 : 0;
   std::vector<int32_t> own(1024 * NSG_ATTN_WORK_INTS);
   nsg_attn_plan_t op{};
   for (;;) {
@@ -186,56 +211,82 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
     if (!grow) return rc;
     own.resize(own.size() * 4);
   }
-  // ---- the prefix tiles ----
-  int64_t most = 0;
-  for (int g = 0; g < num_groups; ++g) {
-    NSG_CHECK_ARG(groups[g] <= groups[g + 1], "group %d: decreasing group_indptr", g);
-    const int np = pkv[g + 1] - pkv[g];
-    NSG_CHECK_ARG(np >= 0, "group %d: decreasing prefix_kv_indptr", g);
-    NSG_CHECK_ARG(np == 0 || (plast[g] >= 1 && plast[g] <= page_size),
-                  "group %d: prefix last_page_len %d outside [1, %d]", g, plast[g], page_size);
-    NSG_CHECK_ARG(np <= kAll / page_size, "group %d: prefix of %d pages", g, np);
-    most = std::max<int64_t>(most, (int64_t)(qo[groups[g + 1]] - qo[groups[g]]) * G);
-  }
-  if (sz.fixed) most = (int64_t)sz.max_batch * sz.max_q_len * G;
-  const int rows = prefix_rows(most, head_dim);
-  const int T = std::max(1, rows / G);
+  // ---- the prefix tiles: steps per item, of the shares that the longest
+  //      prefix can be cut into those with the least estimated time.  Where the
+  //      own parts take several KV groups, the prefix may go with them in one
+  //      launch of that kernel (tiles of at most 64 rows), if that is estimated
+  //      ahead of launches of their own: 32 decode rows of 32 / 8 heads of 128
+  //      behind 4001 tokens 33 -> 24 us without the merge. ----
   auto prefix_len = [&](int g) {
     const int np = pkv[g + 1] - pkv[g];
     return np ? (np - 1) * page_size + plast[g] : 0;
   };
-  auto tiles_of = [&](int g) { return (qo[groups[g + 1]] - qo[groups[g]] + T - 1) / T; };
-  // Steps per item: of the shares that the longest prefix can be cut into, the
-  // number with the least estimated time (an item's page ids must fit the
-  // kernels' list, the items a fixed list)
+  auto steps_of = [&](int g) { return (int64_t)(prefix_len(g) + kStep - 1) / kStep; };
+  auto tiles_of = [&](int g, int T) { return (qo[groups[g + 1]] - qo[groups[g]] + T - 1) / T; };
   int64_t longest = 0;
   for (int g = 0; g < num_groups; ++g)
-    if (tiles_of(g)) longest = std::max<int64_t>(longest, (prefix_len(g) + kStep - 1) / kStep);
+    if (tiles_of(g, 1)) longest = std::max(longest, steps_of(g));
+  // an item's page ids must fit the kernels' list
   const int64_t by_pages =
       std::max<int64_t>(1, (int64_t)(kMaxItemPages - 2) * page_size / kStep);
-  const int64_t fewest = (longest + by_pages - 1) / by_pages;
-  const TileFit fit = tile_fit(rows, head_dim);
-  int64_t chunk = 1;
-  double best = -1;
-  for (int64_t n = std::max<int64_t>(1, fewest); n <= std::max(fewest, std::min<int64_t>(longest, 64));
-       ++n) {
-    const int64_t c = (longest + n - 1) / n;
-    int64_t items = 0;
-    for (int g = 0; g < num_groups; ++g)
-      items += tiles_of(g) * (((prefix_len(g) + kStep - 1) / kStep + c - 1) / c);
-    if (sz.fixed && items > sz.max_prefix_work && best >= 0) break;
-    const double us = tile_us(fit, items, c, (int)n, (int)std::min<int64_t>(rows, most), head_dim,
-                              Hkv, num_cus);
-    if (best < 0 || us < best) {
-      best = us;
-      chunk = c;
+  const int64_t fewest = std::max<int64_t>(1, (longest + by_pages - 1) / by_pages);
+  int64_t own_steps = 0, own_items = 0, own_longest = 0;
+  for (int i = 0; i < op.num_work; ++i) {
+    const int32_t* w = own.data() + (size_t)i * NSG_ATTN_WORK_INTS;
+    const int64_t n = (w[5] - w[4] + kStep - 1) / kStep;
+    own_steps += n;
+    own_items += w[1] > 0;
+    own_longest = std::max(own_longest, n);
+  }
+  struct Choice {
+    double us = -1;
+    int64_t chunk = 1;
+  };
+  auto choose = [&](int rows, bool joint) {
+    Choice best;
+    const TileFit fit = tile_fit(rows, head_dim);
+    const int T = std::max(1, rows / G), real_rows = (int)std::min<int64_t>(rows, most);
+    for (int64_t n = fewest; n <= std::max(fewest, std::min<int64_t>(longest, 64)); ++n) {
+      const int64_t c = std::max<int64_t>(1, (longest + n - 1) / n);
+      int64_t items = 0, steps = 0;
+      for (int g = 0; g < num_groups; ++g) {
+        items += tiles_of(g, T) * ((steps_of(g) + c - 1) / c);
+        steps += tiles_of(g, T) * steps_of(g);
+      }
+      if (sz.fixed && items > sz.max_prefix_work && best.us >= 0) break;
+      const double us =
+          partials_us(items * Hkv, real_rows, head_dim, (int)n) +
+          (joint ? launch_us(fit, (items + own_items) * Hkv, (double)(steps + own_steps) * Hkv,
+                             std::max(c, own_longest), false, num_cus)
+                 : launch_us(fit, items * Hkv, (double)steps * Hkv, c, num_groups == 1, num_cus));
+      if (best.us < 0 || us < best.us) best = {us, c};
+    }
+    return best;
+  };
+  int rows = prefix_rows(most, head_dim);
+  Choice choice = choose(rows, false);
+  bool one_launch = false;
+  if (op.kv_groups > 1) {
+    const int joint_rows =
+        std::max(op.row_tiles * 16, prefix_rows(std::min<int64_t>(most, 64), head_dim));
+    const Choice joint = choose(joint_rows, true);
+    const double own_us = launch_us(tile_fit(16, head_dim), own_items * Hkv,
+                                    (double)own_steps * Hkv, own_longest, false, num_cus);
+    // (a fixed plan's shape must not depend on the lengths of one step)
+    one_launch = sz.fixed ? most <= kFixedJointRows : joint.us < choice.us + own_us + kLaunchGap;
+    if (one_launch) {
+      rows = joint_rows;
+      choice = joint;
     }
   }
+  const int64_t chunk = choice.chunk;
+  const int T = std::max(1, rows / G);
+  const int own_rows = one_launch ? rows : op.row_tiles * 16;
   std::vector<int32_t> pre;
   std::vector<int> first(num_groups), splits(num_groups);
   for (int g = 0; g < num_groups; ++g) {
-    const int len = prefix_len(g), tiles = tiles_of(g), q0 = qo[groups[g]], q1 = qo[groups[g + 1]];
-    const int64_t steps = (len + kStep - 1) / kStep;
+    const int len = prefix_len(g), tiles = tiles_of(g, T), q0 = qo[groups[g]], q1 = qo[groups[g + 1]];
+    const int64_t steps = steps_of(g);
     const int ns = (int)((steps + chunk - 1) / chunk);
     first[g] = (int)(pre.size() / NSG_ATTN_WORK_INTS);
     splits[g] = ns;
@@ -253,32 +304,42 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
   }
   // ---- merge items: one per query tile of the own parts, whose splits are
   //      consecutive items ----
+  const int pre_slots = sz.fixed ? sz.max_prefix_work : n_pre;
+  const int own0 = one_launch ? pre_slots : 0;  // first own item among the partials
   std::vector<int32_t> merge;
   int g = 0;
   for (int i = 0; i < op.num_work;) {
     int32_t* w = own.data() + (size_t)i * NSG_ATTN_WORK_INTS;
     if (w[1] == 0) break;  // padding
     const int ns = std::max(1, w[6]);
-    for (int s = 0; s < ns; ++s) w[(size_t)s * NSG_ATTN_WORK_INTS + 6] = std::max(2, ns);
+    for (int s = 0; s < ns; ++s) {
+      w[(size_t)s * NSG_ATTN_WORK_INTS + 3] += pkv[num_groups];  // after the prefixes' page ids
+      w[(size_t)s * NSG_ATTN_WORK_INTS + 6] = std::max(2, ns);
+    }
     // (tiles need not come in the requests' order)
     g = (int)(std::upper_bound(groups, groups + num_groups + 1, 0,
                                [&](int, int32_t b) { return qo[b] > w[0]; }) -
               groups) - 1;
-    merge.insert(merge.end(), {w[0], w[1], i, ns, first[g], splits[g], qo[groups[g]], 0});
+    merge.insert(merge.end(), {w[0], w[1], i + own0, ns, first[g], splits[g], qo[groups[g]], 0});
     i += ns;
   }
   const int n_merge = (int)(merge.size() / NSG_ATTN_WORK_INTS);
   plan->own = op;
-  plan->num_prefix_work = sz.fixed ? sz.max_prefix_work : n_pre;
+  plan->num_prefix_work = pre_slots;
   plan->num_merge = sz.fixed ? sz.max_merge : n_merge;
   plan->prefix_rows = rows;
   plan->prefix_tile_tokens = T;
   const int64_t q_rows = sz.fixed ? (int64_t)sz.max_batch * sz.max_q_len : qo[batch];
   plan->merge_lanes = q_rows * Hq * (head_dim / 8) <= 65536 ? 4 : 1;
   plan->prefix_kv_groups = rows <= 64 && page_size >= 16 ? (head_dim == 64 ? 4 : 2) : 1;
+  plan->one_launch = one_launch;
+  plan->own_rows = own_rows;
   const int64_t row_bytes = (int64_t)Hkv * (head_dim + 4) * 4;
-  plan->prefix_partials = kHeader + (int64_t)op.num_work * op.row_tiles * 16 * row_bytes;
-  plan->workspace_bytes = plan->prefix_partials + (int64_t)plan->num_prefix_work * rows * row_bytes;
+  const int64_t own_bytes = (int64_t)op.num_work * own_rows * row_bytes;
+  const int64_t pre_bytes = (int64_t)pre_slots * rows * row_bytes;
+  // (one launch: the prefix items come first, in the list and among the partials)
+  plan->prefix_partials = kHeader + (one_launch ? 0 : own_bytes);
+  plan->workspace_bytes = kHeader + own_bytes + pre_bytes;
   const int64_t items = (int64_t)op.num_work + plan->num_prefix_work + plan->num_merge;
   if (sz.fixed && n_merge > sz.max_merge) {
     set_error("plan needs %d merge items, the fixed list holds %d", n_merge, sz.max_merge);
@@ -294,8 +355,9 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
               0);
     work_h += (size_t)slots * NSG_ATTN_WORK_INTS;
   };
+  if (one_launch) put(pre, n_pre, pre_slots);
   put(own, op.num_work, op.num_work);
-  put(pre, n_pre, plan->num_prefix_work);
+  if (!one_launch) put(pre, n_pre, pre_slots);
   put(merge, n_merge, plan->num_merge);
   clear_error();
   return NSG_OK;
@@ -349,7 +411,9 @@ extern "C" int32_t nsg_prefix_attn_fixed_capacity(int32_t batch, int32_t max_q_l
   if (num_cus <= 0) num_cus = 256;
   const int G = num_qo_heads / num_kv_heads;
   const int64_t rows_all = (int64_t)batch * max_q_len * G;
-  const int rows = prefix_rows(rows_all, head_dim);
+  // (the lowest tiles such a plan takes)
+  const int rows = prefix_rows(rows_all <= kFixedJointRows ? std::min<int64_t>(rows_all, 64)
+                                                           : rows_all, head_dim);
   const int T = std::max(1, rows / G);
   // tiles: one more per group for its last, partly filled one; shares: the
   // target, one more per tile for rounding, or what an item's page list forces
@@ -393,7 +457,6 @@ extern "C" int32_t nsg_prefix_attn_plan_fixed(
 extern "C" int32_t nsg_prefix_attn_run(const nsg_prefix_attn_plan_t* plan, const int32_t* work_d,
                                        const void* q, const void* k_cache, const void* v_cache,
                                        const void* kv_scale, void* out,
-                                       const int32_t* prefix_kv_indices,
                                        const int32_t* kv_indices, int32_t page_size,
                                        int32_t num_pages, float sm_scale, int32_t causal,
                                        void* workspace, int64_t workspace_bytes,
@@ -403,8 +466,7 @@ extern "C" int32_t nsg_prefix_attn_run(const nsg_prefix_attn_plan_t* plan, const
     clear_error();
     return NSG_OK;
   }
-  NSG_CHECK_ARG(work_d && q && k_cache && v_cache && out && kv_indices && workspace &&
-                    (prefix_kv_indices || plan->num_prefix_work == 0),
+  NSG_CHECK_ARG(work_d && q && k_cache && v_cache && out && kv_indices && workspace,
                 "null pointer argument");
   NSG_CHECK_ARG(page_size > 0 && (page_size & (page_size - 1)) == 0,
                 "page_size %d must be a power of two", page_size);
@@ -453,31 +515,28 @@ extern "C" int32_t nsg_prefix_attn_run(const nsg_prefix_attn_plan_t* plan, const
                  : launch_tiles_part(pl.head_dim, pl.row_tiles / 2, pl.num_work, prm, s);
     return (fp8 ? launch_verify_attn_fp8 : launch_verify_attn)(&pl, prm, s);
   };
-  // own parts
   prm.work = work_d;
-  prm.num_work = own.num_work;
   prm.kv_indices = kv_indices;
   prm.partials = reinterpret_cast<float*>(ws + kHeader);
-  if (int32_t rc = launch(own)) return rc;
-  // prefix tiles
-  const int* work_p = work_d + (size_t)own.num_work * NSG_ATTN_WORK_INTS;
-  if (plan->num_prefix_work > 0) {
-    nsg_attn_plan_t pp = own;
-    pp.num_work = plan->num_prefix_work;
-    pp.row_tiles = plan->prefix_rows / 16;
-    pp.kv_groups = plan->prefix_kv_groups;
-    prm.work = work_p;
-    prm.num_work = pp.num_work;
-    prm.kv_indices = prefix_kv_indices;
+  nsg_attn_plan_t pl = own;
+  pl.num_work = own.num_work + (plan->one_launch ? plan->num_prefix_work : 0);
+  pl.row_tiles = plan->own_rows / 16;
+  prm.num_work = pl.num_work;
+  if (int32_t rc = launch(pl)) return rc;
+  if (!plan->one_launch && plan->num_prefix_work > 0) {
+    prm.work = work_d + (size_t)own.num_work * NSG_ATTN_WORK_INTS;
     prm.partials = reinterpret_cast<float*>(ws + plan->prefix_partials);
-    if (int32_t rc = launch(pp)) return rc;
+    pl.num_work = prm.num_work = plan->num_prefix_work;
+    pl.row_tiles = plan->prefix_rows / 16;
+    pl.kv_groups = plan->prefix_kv_groups;
+    if (int32_t rc = launch(pl)) return rc;
   }
   MergeParams m{};
-  m.merge = work_p + (size_t)plan->num_prefix_work * NSG_ATTN_WORK_INTS;
+  m.merge = work_d + (size_t)(own.num_work + plan->num_prefix_work) * NSG_ATTN_WORK_INTS;
   m.own = reinterpret_cast<const float*>(ws + kHeader);
   m.prefix = reinterpret_cast<const float*>(ws + plan->prefix_partials);
   m.out = prm.out;
-  m.own_rows = own.row_tiles * 16;
+  m.own_rows = plan->own_rows;
   m.prefix_rows = plan->prefix_rows;
   m.prefix_tokens = plan->prefix_tile_tokens;
   m.Hq = prm.Hq;

@@ -457,10 +457,9 @@ class SharedPrefixAttentionWrapper:
                            int(max_prefix_pages), int(max_kv_len))
             self._caps = None
             self._fixed_shape = None
-            self._idx = torch.zeros(max(1, int(max_pages)), dtype=torch.int32,
+            self._max_ids = (int(max_prefix_pages) * int(max_groups), int(max_pages))
+            self._idx = torch.zeros(max(1, sum(self._max_ids)), dtype=torch.int32,
                                     device=self._device)
-            self._pidx = torch.zeros(max(1, int(max_prefix_pages) * int(max_groups)),
-                                     dtype=torch.int32, device=self._device)
         # index and work arrays of plans that a graph captured: it reads them
         # for as long as it lives
         self._captured: list = []
@@ -485,14 +484,14 @@ class SharedPrefixAttentionWrapper:
         if len(idx) < ptr[-1] or len(pidx) < pptr[-1]:
             raise ValueError(f"{len(idx)} / {len(pidx)} page ids, the indptr arrays end at "
                              f"{ptr[-1]} / {pptr[-1]}")
-        idx, pidx = idx[:ptr[-1]], pidx[:pptr[-1]]
+        ids = np.concatenate([pidx[:pptr[-1]], idx[:ptr[-1]]])     # the prefixes' first
         lib = _lib()
         pl = PrefixAttnPlan()
         args = (qo.ctypes.data, grp.ctypes.data, n, pptr.ctypes.data, plast.ctypes.data,
                 ptr.ctypes.data, last.ctypes.data, B, num_qo_heads, num_kv_heads, head_dim_qk,
                 page_size, 1 if causal else 0, self._num_cus)
         if self._graph:
-            work = self._plan_fixed(lib, pl, args, n, idx, pidx)
+            self._plan_fixed(lib, pl, args, n, ids, int(pptr[-1]))
         else:
             cap = 256
             while True:
@@ -506,9 +505,9 @@ class SharedPrefixAttentionWrapper:
                 break
             self._check_ws(pl)
             work = work[:need * NSG_ATTN_WORK_INTS]
-            self._work, self._idx, self._pidx = (
+            self._work, self._idx = (
                 torch.from_numpy(x if len(x) else np.zeros(1, np.int32)).to(self._device)
-                for x in (work, idx, pidx))
+                for x in (work, ids))
         self._plan = pl
         self._kv_dtype = kv_dtype
         self._total_q = int(qo[-1])
@@ -522,7 +521,7 @@ class SharedPrefixAttentionWrapper:
             raise RuntimeError(f"attention workspace too small: plan needs {pl.workspace_bytes} "
                                f"bytes, buffer has {self._ws_bytes}")
 
-    def _plan_fixed(self, lib, pl, args, n_groups, idx, pidx) -> None:
+    def _plan_fixed(self, lib, pl, args, n_groups, ids, n_prefix) -> None:
         mb, mq, mg, mp, mk = self._sizes
         Hq, Hkv, D, P = args[8:12]
         if self._caps is None:
@@ -537,18 +536,17 @@ class SharedPrefixAttentionWrapper:
         if (Hq, Hkv, D, P) != self._fixed_shape:
             raise ValueError(f"graph-mode wrapper holds heads and pages {self._fixed_shape}, "
                              f"plan has {(Hq, Hkv, D, P)}")
-        if n_groups > mg or len(pidx) > self._pidx.numel() or len(idx) > self._idx.numel():
-            raise ValueError(f"{n_groups} groups, {len(pidx)} prefix and {len(idx)} own pages "
-                             f"exceed the buffers ({mg}, {self._pidx.numel()}, "
-                             f"{self._idx.numel()})")
+        if n_groups > mg or n_prefix > self._max_ids[0] or len(ids) - n_prefix > self._max_ids[1]:
+            raise ValueError(f"{n_groups} groups, {n_prefix} prefix and {len(ids) - n_prefix} own "
+                             f"pages exceed the buffers ({mg}, {self._max_ids[0]}, "
+                             f"{self._max_ids[1]})")
         check(lib.nsg_prefix_attn_plan_fixed(*args, mb, mq, mk, *self._caps,
                                              self._work_h.ctypes.data, sum(self._caps),
                                              C.byref(pl)), "nsg_prefix_attn_plan_fixed")
         self._check_ws(pl)
         self._work.copy_(torch.from_numpy(self._work_h))
-        for buf, h in ((self._idx, idx), (self._pidx, pidx)):
-            if len(h):
-                buf[:len(h)].copy_(torch.from_numpy(h))
+        if len(ids):
+            self._idx[:len(ids)].copy_(torch.from_numpy(ids))
 
     @property
     def plan_info(self) -> PrefixAttnPlan:
@@ -588,11 +586,11 @@ class SharedPrefixAttentionWrapper:
         _same_device(self._device, q=q, k_cache=k_cache, v_cache=v_cache, kv_scale=kv_scale,
                      out=out)
         if not self._graph and torch.cuda.is_current_stream_capturing():
-            self._captured.append((self._work, self._idx, self._pidx))
+            self._captured.append((self._work, self._idx))
         _launch(self._device, _lib().nsg_prefix_attn_run, "nsg_prefix_attn_run",
                 C.byref(self._plan), self._work.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
-                v_cache.data_ptr(), _ptr(kv_scale), out.data_ptr(), self._pidx.data_ptr(),
-                self._idx.data_ptr(), self._page_size, k_cache.shape[0], self._sm_scale,
+                v_cache.data_ptr(), _ptr(kv_scale), out.data_ptr(), self._idx.data_ptr(),
+                self._page_size, k_cache.shape[0], self._sm_scale,
                 1 if self._causal else 0, self._ws.data_ptr(), self._ws_bytes)
         return out
 

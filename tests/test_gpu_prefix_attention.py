@@ -94,22 +94,25 @@ def test_groups_of_all_kinds(heads, P, fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
-@pytest.mark.parametrize("heads,n,q,prefix", [
-    ((32, 8, 128), 3, 1, 2500),      # 12 rows: one 16-row tile
-    ((32, 8, 128), 13, 1, 1999),     # 52 rows: four of them
-    ((14, 2, 64), 3, 5, 1111),       # 105 rows: a 128-row tile
-    ((32, 8, 128), 25, 1, 1500),     # 100 rows, head dim 128
-    ((32, 8, 128), 30, 9, 1500),     # 1080 rows: 256-row tiles, the last one partly filled
-    ((14, 2, 64), 33, 5, 700),       # 1155 rows: 128-row tiles
+@pytest.mark.parametrize("heads,n,q,prefix,P,rows", [
+    ((32, 8, 128), 3, 1, 2500, 16, 16),      # one launch with the own parts: 12 rows
+    ((32, 8, 128), 13, 1, 1999, 16, 64),     # ... 52
+    ((14, 2, 64), 3, 5, 1111, 16, 64),       # ... 105: two tiles of 64
+    ((48, 1, 64), 1, 1, 999, 16, 48),        # ... own tiles taller than 16 rows
+    ((32, 8, 128), 3, 1, 2500, 8, 16),       # small pages: launches of their own
+    ((32, 8, 128), 13, 1, 1999, 8, 64),
+    ((14, 2, 64), 3, 5, 1111, 8, 128),       # ... 105 rows: the 128-row tile
+    ((32, 8, 128), 25, 1, 1500, 8, 128),
+    ((32, 8, 128), 30, 9, 1500, 16, 256),    # 1080 rows: 256-row tiles, the last partly filled
+    ((14, 2, 64), 33, 5, 700, 8, 128),       # 1155 rows: 128-row tiles
 ])
-def test_tile_shapes(heads, n, q, prefix, fp8):
+def test_tile_shapes(heads, n, q, prefix, P, rows, fp8):
     rng = np.random.default_rng(n)
     c = dict(q=[q] * n, kv=[int(q + x) for x in rng.integers(0, 150, n)], groups=[0, n],
              prefix=[prefix])
-    w = _case(n, c, heads, 16, fp8)
-    rows = n * q * heads[0] // heads[1]
-    want = (rows + 15) // 16 * 16 if rows <= 64 else 128 if rows <= 128 or heads[2] == 64 else 256
-    assert w.plan_info.prefix_rows == want
+    pl = _case(n, c, heads, P, fp8).plan_info
+    assert pl.prefix_rows == rows
+    assert pl.one_launch == (P == 16 and rows <= 64)
 
 
 @pytest.mark.parametrize("fp8", [False, True])
@@ -187,17 +190,17 @@ def test_agrees_with_the_per_request_wrapper(fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
-@pytest.mark.parametrize("max_kv_len", [0, 800])
-def test_graph_mode_replays_after_each_plan(fp8, max_kv_len):
+@pytest.mark.parametrize("max_kv_len,Hq", [(0, 14), (800, 14), (800, 4)])
+def test_graph_mode_replays_after_each_plan(fp8, max_kv_len, Hq):
     """One captured run; requests grow, leave and change groups between the
     replays; rows past the plan's stay as they were."""
     rng = np.random.default_rng(6)
-    heads, P, B, mq = (14, 2, 64), 16, 8, 5
+    heads, P, B, mq = (Hq, 2, 64), 16, 8, 5
     pages = 500
     caches, sc, k, v = _pool(rng, fp8, pages, P, 2, 64)
     w = _wrapper(use_cuda_graph=True, max_batch=B, max_q_len=mq, max_groups=3,
                  max_prefix_pages=100, max_pages=420, max_kv_len=max_kv_len)
-    qd = torch.zeros(B * mq, 14, 64, device="cuda", dtype=BF16)
+    qd = torch.zeros(B * mq, Hq, 64, device="cuda", dtype=BF16)
     out = torch.zeros_like(qd)
     graph = None
     for c in (dict(q=[5] * 8, kv=[5 + i for i in range(8)], groups=[0, 8], prefix=[1600]),
@@ -207,7 +210,7 @@ def test_graph_mode_replays_after_each_plan(fp8, max_kv_len):
         ptabs, tabs = _tables(rng, c, P, pages)
         _plan(w, c, ptabs, tabs, heads, P, fp8)
         n = sum(c["q"])
-        q = fc.bf16(rng.standard_normal((B * mq, 14, 64)))
+        q = fc.bf16(rng.standard_normal((B * mq, Hq, 64)))
         qd.copy_(torch.from_numpy(q))
         if graph is None:
             side = torch.cuda.Stream()
@@ -223,6 +226,7 @@ def test_graph_mode_replays_after_each_plan(fp8, max_kv_len):
         graph.replay()
         torch.cuda.synchronize()
         assert w.check_flags() == 0
+        assert w.plan_info.one_launch == (max_kv_len > 0)    # with the own parts
         fc.check(out[:n], *_want(q[:n], c, ptabs, tabs, k, v))
         assert (out[n:] == 9.0).all()
 

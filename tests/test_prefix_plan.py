@@ -32,7 +32,9 @@ def _plan(lib, q_lens, kv_lens, groups, prefix_lens, Hq=32, Hkv=8, D=128, P=16, 
         rc = lib.nsg_prefix_attn_plan_fixed(*args, *fixed, work.ctypes.data, cap, C.byref(pl))
     w = work.reshape(-1, NSG_ATTN_WORK_INTS)
     a, b = pl.own.num_work, pl.own.num_work + pl.num_prefix_work
-    return rc, pl, (w[:a], w[a:b], w[b:b + pl.num_merge]), (qo, pptr, ptr)
+    n = pl.num_prefix_work
+    own, pre = (w[n:b], w[:n]) if pl.one_launch else (w[:a], w[a:b])
+    return rc, pl, (own, pre, w[b:b + pl.num_merge]), (qo, pptr, ptr)
 
 
 def _check(pl, items, arrays, q_lens, kv_lens, groups, prefix_lens, G, P, causal=True):
@@ -48,12 +50,14 @@ def _check(pl, items, arrays, q_lens, kv_lens, groups, prefix_lens, G, P, causal
             b += 1
         g = int(np.searchsorted(groups, b, side="right") - 1)
         seen[qs:qs + qn] += 1
+        if pl.one_launch:                             # partials: the prefix items' first
+            wi0 -= pl.num_prefix_work
         assert qs + qn <= qo[b + 1] and qn <= T and g0 == qo[groups[g]]
         L = kv_lens[b]
         end = L - q_lens[b] + (qs - qo[b]) + qn if causal else L
         rng = []
         for w in own[wi0:wi0 + ns]:
-            assert (w[0], w[1], w[3]) == (qs, qn, ptr[b]) and w[6] >= 2
+            assert (w[0], w[1], w[3]) == (qs, qn, ptr[b] + pptr[-1]) and w[6] >= 2
             assert w[2] == (L - q_lens[b] + qs - qo[b] if causal else L - 1)
             rng.append((w[4], w[5]))
         assert rng[0][0] == 0 and rng[-1][1] == end
@@ -85,7 +89,9 @@ def test_every_row_meets_every_token_once(lib, Hq, Hkv, D, P, cus):
         assert rc == 0, lib.nsg_last_error()
         _check(pl, items, arrays, q_lens, kv_lens, groups, pre, Hq // Hkv, P)
         rows = 4 * Hkv * (D + 4)
-        assert pl.workspace_bytes >= 256 + rows * (pl.own.num_work * pl.own.row_tiles * 16
+        assert pl.own_rows >= pl.own.row_tiles * 16
+        assert not pl.one_launch or pl.own_rows == pl.prefix_rows
+        assert pl.workspace_bytes >= 256 + rows * (pl.own.num_work * pl.own_rows
                                                    + pl.num_prefix_work * pl.prefix_rows)
 
 
@@ -102,8 +108,11 @@ def test_prompts_and_not_causal(lib):
 
 @pytest.mark.parametrize("Hq,Hkv,D,P", [(32, 8, 128, 16), (14, 2, 64, 16), (14, 2, 64, 1)])
 @pytest.mark.parametrize("max_kv", [0, 900])
-def test_fixed_plans_keep_one_grid(lib, Hq, Hkv, D, P, max_kv):
+@pytest.mark.parametrize("small", [False, True])
+def test_fixed_plans_keep_one_grid(lib, Hq, Hkv, D, P, max_kv, small):
     B, mq, mg, pages = 12, 5, 3, -(-6000 // P)
+    if small:
+        B, mq = 12, 1
     c = [C.c_int32(0) for _ in range(3)]
     assert lib.nsg_prefix_attn_fixed_capacity(B, mq, mg, Hq, Hkv, D, 256, max_kv, pages, P,
                                               *map(C.byref, c)) == 0
@@ -125,6 +134,8 @@ def test_fixed_plans_keep_one_grid(lib, Hq, Hkv, D, P, max_kv):
             used = np.flatnonzero(part[:, 1])
             assert not part[used[-1] + 1 if len(used) else 0:].any()
     assert len(shapes) == 1
+    assert pl.one_launch == (B * mq * Hq // Hkv <= 512 and max_kv > 0 and P >= 16
+                             and pl.own.kv_groups > 1)
     rc, *_ = _plan(lib, [1] * 13, [5] * 13, [0, 13], [10], Hq, Hkv, D, P, fixed=fixed)
     assert rc == 1 and b"exceeds" in lib.nsg_last_error()
 
@@ -138,6 +149,7 @@ def test_refusals(lib):
     assert "group_indptr" in err([1, 1], [5, 6], [0, 1], [40])[1]
     assert "group_indptr" in err([1, 1], [5, 6], [1, 2], [40])[1]
     assert "decreasing" in err([1, 1], [5, 6], [0, 2, 1, 2], [40, 1, 1])[1]
+    assert "decreasing" in err([1, 1], [5, 6], [0, 50, 2], [40, 1])[1]
     assert "empty KV" in err([1, 1], [5, 0], [0, 2], [40])[1]
     assert "query length" in err([1, 9], [5, 6], [0, 2], [40])[1]
     assert err(*ok, D=96)[0] == 2 and err(*ok, Hq=9)[0] == 1
@@ -160,14 +172,14 @@ OK = 0x1000
 
 
 @pytest.mark.parametrize("change,rc,match", [
-    (dict(q=None), 1, "null"), (dict(pidx=None), 1, "null"), (dict(page=5), 1, "page_size"),
+    (dict(q=None), 1, "null"), (dict(idx=None), 1, "null"), (dict(page=5), 1, "page_size"),
     (dict(page=8), 1, "KV groups"), (dict(num_pages=0), 1, "num_pages"), (dict(sm=-1.0), 1, "sm"),
     (dict(out=OK + 8), 1, "aligned"), (dict(ws=100), 3, "workspace")])
 def test_run_refuses(lib, change, rc, match):
     r, pl, *_ = _plan(lib, [1, 1], [5, 6], [0, 2], [40])
     assert r == 0 and pl.own.kv_groups > 1
-    a = dict(q=OK, out=OK, pidx=OK, page=16, num_pages=9, sm=0.1, ws=pl.workspace_bytes)
+    a = dict(q=OK, out=OK, idx=OK, page=16, num_pages=9, sm=0.1, ws=pl.workspace_bytes)
     a.update(change)
-    got = lib.nsg_prefix_attn_run(C.byref(pl), OK, a["q"], OK, OK, None, a["out"], a["pidx"], OK,
+    got = lib.nsg_prefix_attn_run(C.byref(pl), OK, a["q"], OK, OK, None, a["out"], a["idx"],
                                   a["page"], a["num_pages"], a["sm"], 1, OK, a["ws"], None)
     assert got == rc and match in lib.nsg_last_error().decode()
