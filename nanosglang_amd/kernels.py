@@ -52,11 +52,15 @@ def _require_gpu(t: torch.Tensor, name: str) -> None:
 def _launch(device: torch.device, fn, what: str, *args) -> None:
     """``fn(*args, stream)`` on ``device``'s current stream, with that device
     current for the call."""
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, _stream_ptr(device)), what)
+    index = device.index
+    if index == torch.cuda.current_device():
+        # (the raw handle: a Stream object costs more than the checks here)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            check(fn(*args, _stream_ptr(device)), what)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, what)
 
 
 def _same_device(device: torch.device, **tensors: torch.Tensor | None) -> None:
@@ -907,21 +911,28 @@ def _check_fp8_pool(k_cache, v_cache, kv_scale, num_kv_heads: int, head_dim: int
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if t is None:
             raise ValueError(f"{name} is missing")
-        _require_gpu(t, name)
+        if t.device != device:
+            _require_gpu(t, name)
+            _same_device(device, **{name: t})
         if t.dtype != FP8:
             raise TypeError(f"{name} must be float8_e4m3fn, got {t.dtype}")
         if t.dim() != 4 or not t.is_contiguous():
             raise ValueError(f"{name} must be one layer's contiguous (pages, P, Hkv, D) pool")
-    if v_cache.shape != k_cache.shape or tuple(k_cache.shape[2:]) != (num_kv_heads, head_dim):
+    pages, P, heads, dim = k_cache.shape
+    if v_cache.shape != k_cache.shape or heads != num_kv_heads or dim != head_dim:
         raise ValueError(f"caches {tuple(k_cache.shape)} / {tuple(v_cache.shape)} do not match "
                          f"(pages, P, {num_kv_heads}, {head_dim})")
     _check_kv_scale(kv_scale, k_cache)
-    _same_device(device, k_cache=k_cache, v_cache=v_cache, kv_scale=kv_scale)
-    return k_cache.shape[1], k_cache.shape[0] * k_cache.shape[1]
+    if kv_scale.device != device:
+        _same_device(device, kv_scale=kv_scale)
+    return P, pages * P
 
 
 def _token_index(t, name: str, T: int, device: torch.device) -> torch.Tensor:
     """Contiguous int64 (T,) on ``device``."""
+    if (t.device == device and t.dtype == torch.int64 and t.dim() == 1 and t.shape[0] == T
+            and t.is_contiguous()):
+        return t
     _require_gpu(t, name)
     _same_device(device, **{name: t})
     if t.dtype not in (torch.int64, torch.int32) or t.numel() != T:
