@@ -191,10 +191,11 @@ int32_t fill_impl(const int32_t* page_table, int64_t page_table_stride, const in
     int32_t* work = o.work + (size_t)a * o.work_stride;
     const nsg_attn_plan_t& p0 = plans[0];
     if (a >= 1 && a < k && p0.q_tile_tokens == 1 && p0.max_splits == 1 && p0.num_merge == 0 &&
-        p0.num_work == S && p0.num_groups == S) {
+        p0.num_work == S && p0.num_groups == S && p0.kv_groups > 1) {
       // a later draft call: one query token per row, so the plan of draft
       // call 0 with each row's KV range moved (its work item n is row n, one
-      // KV split): the planner would write exactly this
+      // KV split, as several KV groups have them; one group's go longest
+      // first): the planner would write exactly this
       plans[a] = p0;
       for (int j = 0; j < S; ++j) {
         const int32_t L = (kvp[j + 1] - kvp[j] - 1) * P + last[j];
