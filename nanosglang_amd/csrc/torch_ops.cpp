@@ -19,6 +19,10 @@
 //   nsg::sample                 temperature / top-k / top-p, one token per row
 //   nsg::kv_write, nsg::rope_kv_write
 //                               K / V rows (after RoPE) into flat KV slots
+//   nsg::kv_write_fp8, nsg::rope_kv_write_fp8, nsg::kv_read_fp8,
+//   nsg::verify_attention_fp8, nsg::verify_attention_run_fp8
+//                               the same over the 8-bit pool, and its rows back
+//   nsg::shared_prefix_attention  groups of requests behind common prefixes
 //
 // Host (CPU) tensors given to a device operator are rejected with an error;
 // there is no CPU implementation.  Shape-only (fake) implementations are
@@ -426,7 +430,8 @@ void kv_write(const Tensor& k, const Tensor& v, const Tensor& slots, const Tenso
   const int64_t T = k.size(0), Hkv = k.size(1), D = k.size(2);
   TORCH_CHECK_VALUE(k.stride(2) == 1 && k.stride(1) == D,
                     "each K/V row must be a contiguous (Hkv, D) block");
-  TORCH_CHECK(k.scalar_type() == at::kBFloat16 && k_cache.scalar_type() == at::kBFloat16,
+  TORCH_CHECK(k.scalar_type() == at::kBFloat16 && k_cache.scalar_type() == at::kBFloat16 &&
+                  v_cache.scalar_type() == at::kBFloat16,
               "K/V and caches must be bfloat16");
   TORCH_CHECK_VALUE(k_cache.is_contiguous() && v_cache.is_contiguous(), "caches must be contiguous");
   TORCH_CHECK_VALUE(k_cache.size(-2) == Hkv && k_cache.size(-1) == D,
@@ -453,6 +458,9 @@ Tensor rope_kv_write(const Tensor& qkv, int64_t num_qo_heads, int64_t num_kv_hea
                     "qkv must be bfloat16 (T, (Hq + 2 Hkv) D) with unit inner stride");
   require(cos_table, "cos_table", at::kFloat);
   require(sin_table, "sin_table", at::kFloat);
+  TORCH_CHECK(k_cache.scalar_type() != at::kFloat8_e4m3fn &&
+                  v_cache.scalar_type() != at::kFloat8_e4m3fn,
+              "the caches are an 8-bit pool: use rope_kv_write_fp8");
   const int64_t T = qkv.size(0);
   const DeviceGuard guard(qkv.device());
   Tensor q_out = at::empty({T, num_qo_heads, head_dim}, qkv.options());
@@ -470,6 +478,267 @@ Tensor rope_kv_write(const Tensor& qkv, int64_t num_qo_heads, int64_t num_kv_hea
                                  stream_of(qkv)),
                "nsg_rope_kv_write");
   return q_out;
+}
+
+// ---- the 8-bit KV pool and shared prefixes ----
+
+// One layer's 8-bit pool: e4m3 codes (pages, P, Hkv, D) and their scales
+// uint8 (pages, Hkv, 2, P), all on `dev`.
+void require_fp8_pool(const Tensor& k_cache, const Tensor& v_cache, const Tensor& kv_scale,
+                      const at::Device& dev) {
+  require(k_cache, "k_cache", at::kFloat8_e4m3fn);
+  require(v_cache, "v_cache", at::kFloat8_e4m3fn);
+  require(kv_scale, "kv_scale", at::kByte);
+  TORCH_CHECK_VALUE(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes(),
+                    "caches must be one layer's (pages, P, Hkv, D)");
+  const at::IntArrayRef s = k_cache.sizes();
+  TORCH_CHECK_VALUE(kv_scale.sizes() == at::IntArrayRef({s[0], s[2], 2, s[1]}),
+                    "kv_scale must be (pages, Hkv, 2, P)");
+  TORCH_CHECK_VALUE(k_cache.device() == dev && v_cache.device() == dev && kv_scale.device() == dev,
+                    "all tensors must be on ", dev);
+}
+
+// Contiguous int64 copy (or the tensor itself) of T indices on `dev`.
+Tensor token_index(const Tensor& t, const char* name, int64_t T, const at::Device& dev) {
+  require_gpu(t, name);
+  TORCH_CHECK_VALUE(t.device() == dev && t.numel() == T &&
+                        (t.scalar_type() == at::kLong || t.scalar_type() == at::kInt),
+                    name, " must hold ", T, " integers on ", dev);
+  return t.reshape({-1}).to(at::kLong).contiguous();
+}
+
+void kv_write_fp8(const Tensor& k, const Tensor& v, const Tensor& slots, const Tensor& k_cache,
+                  const Tensor& v_cache, const Tensor& kv_scale) {
+  require_gpu(k, "k");
+  require_gpu(v, "v");
+  const at::Device dev = k.device();
+  require_fp8_pool(k_cache, v_cache, kv_scale, dev);
+  TORCH_CHECK_VALUE(k.dim() == 3 && v.sizes() == k.sizes() && v.device() == dev &&
+                        k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16,
+                    "k and v must be bfloat16 (T, Hkv, D) on ", dev);
+  const int64_t T = k.size(0), Hkv = k.size(1), D = k.size(2);
+  TORCH_CHECK_VALUE(k_cache.size(2) == Hkv && k_cache.size(3) == D,
+                    "cache head layout does not match K/V");
+  for (const Tensor& t : {k, v})
+    TORCH_CHECK_VALUE(T == 0 || (t.stride(2) == 1 && (Hkv == 1 || t.stride(1) == D)),
+                      "each K/V row must be a contiguous (Hkv, D) block");
+  const DeviceGuard guard(dev);
+  const Tensor sl = token_index(slots, "slots", T, dev);
+  const int64_t P = k_cache.size(1);
+  check_status(nsg_kv_write_fp8(k.data_ptr(), T > 1 ? k.stride(0) : Hkv * D, v.data_ptr(),
+                                T > 1 ? v.stride(0) : Hkv * D, sl.data_ptr<int64_t>(),
+                                static_cast<int32_t>(T), k_cache.data_ptr(), v_cache.data_ptr(),
+                                kv_scale.data_ptr(), static_cast<int32_t>(Hkv),
+                                static_cast<int32_t>(D), static_cast<int32_t>(P),
+                                k_cache.size(0) * P, stream_of(k)),
+               "nsg_kv_write_fp8");
+}
+
+std::tuple<Tensor, Tensor> kv_read_fp8(const Tensor& slots, const Tensor& k_cache,
+                                       const Tensor& v_cache, const Tensor& kv_scale) {
+  require_gpu(k_cache, "k_cache");
+  const at::Device dev = k_cache.device();
+  require_fp8_pool(k_cache, v_cache, kv_scale, dev);
+  const DeviceGuard guard(dev);
+  const int64_t T = slots.numel(), P = k_cache.size(1), Hkv = k_cache.size(2),
+                D = k_cache.size(3);
+  const Tensor sl = token_index(slots, "slots", T, dev);
+  const auto opt = k_cache.options().dtype(at::kBFloat16);
+  Tensor k = at::empty({T, Hkv, D}, opt), v = at::empty({T, Hkv, D}, opt);
+  check_status(nsg_kv_read_fp8(sl.data_ptr<int64_t>(), static_cast<int32_t>(T),
+                               k_cache.data_ptr(), v_cache.data_ptr(), kv_scale.data_ptr(),
+                               static_cast<int32_t>(Hkv), static_cast<int32_t>(D),
+                               static_cast<int32_t>(P), k_cache.size(0) * P, k.data_ptr(),
+                               v.data_ptr(), stream_of(k_cache)),
+               "nsg_kv_read_fp8");
+  return {k, v};
+}
+
+Tensor rope_kv_write_fp8(const Tensor& qkv, int64_t num_qo_heads, int64_t num_kv_heads,
+                         int64_t head_dim, const Tensor& positions, const Tensor& cos_table,
+                         const Tensor& sin_table, const Tensor& slots, const Tensor& k_cache,
+                         const Tensor& v_cache, const Tensor& kv_scale) {
+  require_gpu(qkv, "qkv");
+  const at::Device dev = qkv.device();
+  require_fp8_pool(k_cache, v_cache, kv_scale, dev);
+  TORCH_CHECK_VALUE(qkv.scalar_type() == at::kBFloat16 && qkv.dim() == 2 && qkv.stride(1) == 1 &&
+                        qkv.size(1) == (num_qo_heads + 2 * num_kv_heads) * head_dim,
+                    "qkv must be bfloat16 (T, (Hq + 2 Hkv) D) with unit inner stride");
+  TORCH_CHECK_VALUE(k_cache.size(2) == num_kv_heads && k_cache.size(3) == head_dim,
+                    "cache head layout does not match the heads");
+  for (const auto& [t, name] : {std::pair<const Tensor&, const char*>{cos_table, "cos_table"},
+                                {sin_table, "sin_table"}}) {
+    require(t, name, at::kFloat);
+    TORCH_CHECK_VALUE(t.dim() == 2 && 2 * t.size(1) == head_dim &&
+                          t.size(0) == cos_table.size(0) && t.device() == dev,
+                      name, " must be (max_position, head_dim / 2) on ", dev);
+  }
+  const int64_t T = qkv.size(0), P = k_cache.size(1);
+  const DeviceGuard guard(dev);
+  const Tensor pos = token_index(positions, "positions", T, dev),
+               sl = token_index(slots, "slots", T, dev);
+  Tensor q_out = at::empty({T, num_qo_heads, head_dim}, qkv.options());
+  check_status(nsg_rope_kv_write_fp8(
+                   qkv.data_ptr(), T > 1 ? qkv.stride(0) : qkv.size(1), pos.data_ptr<int64_t>(),
+                   cos_table.data_ptr<float>(), sin_table.data_ptr<float>(),
+                   static_cast<int32_t>(cos_table.size(0)), sl.data_ptr<int64_t>(),
+                   static_cast<int32_t>(T), static_cast<int32_t>(num_qo_heads),
+                   static_cast<int32_t>(num_kv_heads), static_cast<int32_t>(head_dim),
+                   static_cast<int32_t>(P), q_out.data_ptr(), k_cache.data_ptr(),
+                   v_cache.data_ptr(), kv_scale.data_ptr(), k_cache.size(0) * P, nullptr,
+                   stream_of(qkv)),
+               "nsg_rope_kv_write_fp8");
+  return q_out;
+}
+
+void verify_attention_run_fp8(const Tensor& plan, const Tensor& work, const Tensor& q,
+                              const Tensor& k_cache, const Tensor& v_cache,
+                              const Tensor& kv_scale, const Tensor& paged_kv_indices,
+                              double sm_scale, bool causal, const Tensor& workspace,
+                              const Tensor& out) {
+  require(q, "q", at::kBFloat16);
+  require(out, "out", at::kBFloat16);
+  require(work, "work", at::kInt);
+  require(paged_kv_indices, "paged_kv_indices", at::kInt);
+  require_gpu(workspace, "workspace");
+  const at::Device dev = q.device();
+  require_fp8_pool(k_cache, v_cache, kv_scale, dev);
+  for (const Tensor& t : {out, work, paged_kv_indices, workspace})
+    TORCH_CHECK_VALUE(t.device() == dev, "all tensors must be on ", dev);
+  nsg_attn_plan_t pl;
+  int64_t total_q, nnz, B;
+  read_record(plan, &pl, &total_q, &nnz, &B);
+  TORCH_CHECK_VALUE(q.dim() == 3 && q.size(0) == total_q && q.size(1) == pl.num_qo_heads &&
+                        q.size(2) == pl.head_dim && out.sizes() == q.sizes(),
+                    "q / out must be (", total_q, ", ", pl.num_qo_heads, ", ", pl.head_dim,
+                    ") as planned");
+  TORCH_CHECK_VALUE(k_cache.size(2) == pl.num_kv_heads && k_cache.size(3) == pl.head_dim,
+                    "caches must be (pages, P, ", pl.num_kv_heads, ", ", pl.head_dim, ")");
+  TORCH_CHECK_VALUE(paged_kv_indices.numel() >= nnz, "the plan has ", nnz, " page ids");
+  TORCH_CHECK_VALUE(work.numel() >= static_cast<int64_t>(pl.num_work + pl.num_merge) *
+                                         NSG_ATTN_WORK_INTS,
+                    "work list shorter than the plan");
+  const int64_t wsb = workspace.numel() * workspace.element_size();
+  TORCH_CHECK_VALUE(wsb >= pl.workspace_bytes, "workspace has ", wsb,
+                    " bytes, the plan needs ", pl.workspace_bytes);
+  const DeviceGuard guard(dev);
+  check_status(nsg_attn_run_fp8(&pl, work.data_ptr<int32_t>(), q.data_ptr(), k_cache.data_ptr(),
+                                v_cache.data_ptr(), kv_scale.data_ptr(), out.data_ptr(),
+                                paged_kv_indices.data_ptr<int32_t>(),
+                                static_cast<int32_t>(k_cache.size(1)),
+                                static_cast<int32_t>(k_cache.size(0)),
+                                static_cast<float>(sm_scale), causal ? 1 : 0,
+                                workspace.data_ptr(), wsb, stream_of(q)),
+               "nsg_attn_run_fp8");
+}
+
+Tensor verify_attention_fp8(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                            const Tensor& kv_scale, const Tensor& qo_indptr,
+                            const Tensor& paged_kv_indptr, const Tensor& paged_kv_indices,
+                            const Tensor& paged_kv_last_page_len, bool causal,
+                            optional<double> sm_scale) {
+  require(q, "q", at::kBFloat16);
+  const at::Device dev = q.device();
+  require_fp8_pool(k_cache, v_cache, kv_scale, dev);
+  TORCH_CHECK_VALUE(q.dim() == 3, "q must be (T, Hq, D)");
+  const int64_t D = q.size(2);
+  auto [rec, work_h] = verify_attention_plan(qo_indptr, paged_kv_indptr, paged_kv_last_page_len,
+                                             q.size(1), k_cache.size(2), D, k_cache.size(1),
+                                             causal, kMi355xCus);
+  nsg_attn_plan_t pl;
+  int64_t total_q, nnz, B;
+  read_record(rec, &pl, &total_q, &nnz, &B);
+  const DeviceGuard guard(dev);
+  const Tensor ws = workspace(dev, stream_of(q), kAttnWs,
+                              std::max<int64_t>(128 << 20, pl.workspace_bytes));
+  Tensor out = at::empty_like(q);
+  verify_attention_run_fp8(rec, work_h.to(dev), q, k_cache, v_cache, kv_scale,
+                           paged_kv_indices.to(dev, at::kInt).contiguous(),
+                           sm_scale.has_value() ? *sm_scale
+                                                : 1.0 / std::sqrt(static_cast<double>(D)),
+                           causal, ws, out);
+  return out;
+}
+
+Tensor shared_prefix_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache,
+                               const optional<Tensor>& kv_scale, const Tensor& qo_indptr,
+                               const Tensor& group_indptr, const Tensor& prefix_kv_indptr,
+                               const Tensor& prefix_kv_indices,
+                               const Tensor& prefix_kv_last_page_len,
+                               const Tensor& paged_kv_indptr, const Tensor& paged_kv_indices,
+                               const Tensor& paged_kv_last_page_len, bool causal,
+                               optional<double> sm_scale) {
+  require(q, "q", at::kBFloat16);
+  const at::Device dev = q.device();
+  if (kv_scale.has_value()) {
+    require_fp8_pool(k_cache, v_cache, *kv_scale, dev);
+  } else {
+    require(k_cache, "k_cache", at::kBFloat16);
+    require(v_cache, "v_cache", at::kBFloat16);
+    TORCH_CHECK_VALUE(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes() &&
+                          k_cache.device() == dev && v_cache.device() == dev,
+                      "caches must be (pages, P, Hkv, D) on ", dev);
+  }
+  TORCH_CHECK_VALUE(q.dim() == 3 && k_cache.size(3) == q.size(2),
+                    "q must be (T, Hq, D) with the caches' D");
+  const int64_t D = q.size(2);
+  const Tensor qo = host_i32(qo_indptr), grp = host_i32(group_indptr),
+               pptr = host_i32(prefix_kv_indptr), plast = host_i32(prefix_kv_last_page_len),
+               ptr = host_i32(paged_kv_indptr), last = host_i32(paged_kv_last_page_len);
+  const int64_t B = qo.numel() - 1, n = grp.numel() - 1;
+  TORCH_CHECK_VALUE(B >= 0 && n >= 0 && ptr.numel() == B + 1 && last.numel() == B &&
+                        pptr.numel() == n + 1 && plast.numel() == n,
+                    "qo_indptr, group_indptr, the kv_indptr and last_page_len arrays disagree on "
+                    "batch or groups");
+  const int64_t n_pre = pptr.data_ptr<int32_t>()[n], n_own = ptr.data_ptr<int32_t>()[B];
+  TORCH_CHECK_VALUE(n_pre >= 0 && n_own >= 0 && prefix_kv_indices.numel() >= n_pre &&
+                        paged_kv_indices.numel() >= n_own,
+                    "the indptr arrays end at ", n_pre, " / ", n_own, " page ids");
+  TORCH_CHECK_VALUE(q.size(0) == qo.data_ptr<int32_t>()[B], "q must have qo_indptr[-1] rows");
+  nsg_prefix_attn_plan_t pl{};
+  Tensor work;
+  for (int64_t cap = 256;;) {
+    work = at::zeros({cap * NSG_ATTN_WORK_INTS}, at::TensorOptions().dtype(at::kInt));
+    const int32_t rc = nsg_prefix_attn_plan(
+        qo.data_ptr<int32_t>(), grp.data_ptr<int32_t>(), static_cast<int32_t>(n),
+        pptr.data_ptr<int32_t>(), plast.data_ptr<int32_t>(), ptr.data_ptr<int32_t>(),
+        last.data_ptr<int32_t>(), static_cast<int32_t>(B), static_cast<int32_t>(q.size(1)),
+        static_cast<int32_t>(k_cache.size(2)), static_cast<int32_t>(D),
+        static_cast<int32_t>(k_cache.size(1)), causal ? 1 : 0, kMi355xCus,
+        work.data_ptr<int32_t>(), static_cast<int32_t>(cap), &pl);
+    const int64_t need =
+        static_cast<int64_t>(pl.own.num_work) + pl.num_prefix_work + pl.num_merge;
+    if (rc == NSG_ERR_WORKSPACE && need > cap) {
+      cap = need;
+      continue;
+    }
+    check_status(rc, "nsg_prefix_attn_plan");
+    work = work.narrow(0, 0, std::max<int64_t>(1, need * NSG_ATTN_WORK_INTS));
+    break;
+  }
+  const DeviceGuard guard(dev);
+  // the prefixes' page ids first, then the batch's; never an empty tensor
+  const auto i32 = at::TensorOptions().dtype(at::kInt).device(dev);
+  const Tensor ids = at::zeros({std::max<int64_t>(1, n_pre + n_own)}, i32);
+  if (n_pre)
+    ids.narrow(0, 0, n_pre).copy_(prefix_kv_indices.reshape({-1}).narrow(0, 0, n_pre));
+  if (n_own)
+    ids.narrow(0, n_pre, n_own).copy_(paged_kv_indices.reshape({-1}).narrow(0, 0, n_own));
+  const Tensor work_d = work.to(dev);
+  void* s = stream_of(q);
+  const Tensor ws = workspace(dev, s, kAttnWs, std::max<int64_t>(128 << 20, pl.workspace_bytes));
+  Tensor out = at::empty_like(q);
+  check_status(nsg_prefix_attn_run(
+                   &pl, work_d.data_ptr<int32_t>(), q.data_ptr(), k_cache.data_ptr(),
+                   v_cache.data_ptr(), kv_scale.has_value() ? kv_scale->data_ptr() : nullptr,
+                   out.data_ptr(), ids.data_ptr<int32_t>(), static_cast<int32_t>(k_cache.size(1)),
+                   static_cast<int32_t>(k_cache.size(0)),
+                   static_cast<float>(sm_scale.has_value()
+                                          ? *sm_scale
+                                          : 1.0 / std::sqrt(static_cast<double>(D))),
+                   causal ? 1 : 0, ws.data_ptr(), ws.numel(), s),
+               "nsg_prefix_attn_run");
+  return out;
 }
 
 // ---- host tensors given to the device operators ----
@@ -508,6 +777,30 @@ TORCH_LIBRARY(nsg, m) {
       "rope_kv_write(Tensor qkv, int num_qo_heads, int num_kv_heads, int head_dim, "
       "Tensor positions, Tensor cos_table, Tensor sin_table, Tensor slots, "
       "Tensor(a!) k_cache, Tensor(b!) v_cache) -> Tensor");
+  m.def(
+      "kv_write_fp8(Tensor k, Tensor v, Tensor slots, Tensor(a!) k_cache, Tensor(b!) v_cache, "
+      "Tensor(c!) kv_scale) -> ()");
+  m.def(
+      "kv_read_fp8(Tensor slots, Tensor k_cache, Tensor v_cache, Tensor kv_scale) "
+      "-> (Tensor, Tensor)");
+  m.def(
+      "rope_kv_write_fp8(Tensor qkv, int num_qo_heads, int num_kv_heads, int head_dim, "
+      "Tensor positions, Tensor cos_table, Tensor sin_table, Tensor slots, "
+      "Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) kv_scale) -> Tensor");
+  m.def(
+      "verify_attention_fp8(Tensor q, Tensor k_cache, Tensor v_cache, Tensor kv_scale, "
+      "Tensor qo_indptr, Tensor paged_kv_indptr, Tensor paged_kv_indices, "
+      "Tensor paged_kv_last_page_len, bool causal=True, float? sm_scale=None) -> Tensor");
+  m.def(
+      "verify_attention_run_fp8(Tensor plan, Tensor work, Tensor q, Tensor k_cache, "
+      "Tensor v_cache, Tensor kv_scale, Tensor paged_kv_indices, float sm_scale, bool causal, "
+      "Tensor(a!) workspace, Tensor(b!) out) -> ()");
+  m.def(
+      "shared_prefix_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor? kv_scale, "
+      "Tensor qo_indptr, Tensor group_indptr, Tensor prefix_kv_indptr, "
+      "Tensor prefix_kv_indices, Tensor prefix_kv_last_page_len, Tensor paged_kv_indptr, "
+      "Tensor paged_kv_indices, Tensor paged_kv_last_page_len, bool causal=True, "
+      "float? sm_scale=None) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(nsg, CUDA, m) {
@@ -518,6 +811,12 @@ TORCH_LIBRARY_IMPL(nsg, CUDA, m) {
   m.impl("sample", &sample);
   m.impl("kv_write", &kv_write);
   m.impl("rope_kv_write", &rope_kv_write);
+  m.impl("kv_write_fp8", &kv_write_fp8);
+  m.impl("kv_read_fp8", &kv_read_fp8);
+  m.impl("rope_kv_write_fp8", &rope_kv_write_fp8);
+  m.impl("verify_attention_fp8", &verify_attention_fp8);
+  m.impl("verify_attention_run_fp8", &verify_attention_run_fp8);
+  m.impl("shared_prefix_attention", &shared_prefix_attention);
 }
 
 TORCH_LIBRARY_IMPL(nsg, CPU, m) {
@@ -545,5 +844,31 @@ TORCH_LIBRARY_IMPL(nsg, CPU, m) {
          [](const Tensor&, int64_t, int64_t, int64_t, const Tensor&, const Tensor&, const Tensor&,
             const Tensor&, const Tensor&, const Tensor&) -> Tensor {
            host_tensors("rope_kv_write");
+         });
+  m.impl("kv_write_fp8", [](const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                            const Tensor&, const Tensor&) { host_tensors("kv_write_fp8"); });
+  m.impl("kv_read_fp8",
+         [](const Tensor&, const Tensor&, const Tensor&, const Tensor&)
+             -> std::tuple<Tensor, Tensor> { host_tensors("kv_read_fp8"); });
+  m.impl("rope_kv_write_fp8",
+         [](const Tensor&, int64_t, int64_t, int64_t, const Tensor&, const Tensor&, const Tensor&,
+            const Tensor&, const Tensor&, const Tensor&, const Tensor&) -> Tensor {
+           host_tensors("rope_kv_write_fp8");
+         });
+  m.impl("verify_attention_fp8",
+         [](const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+            const Tensor&, const Tensor&, const Tensor&, bool, optional<double>) -> Tensor {
+           host_tensors("verify_attention_fp8");
+         });
+  m.impl("verify_attention_run_fp8",
+         [](const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+            const Tensor&, const Tensor&, double, bool, const Tensor&, const Tensor&) {
+           host_tensors("verify_attention_run_fp8");
+         });
+  m.impl("shared_prefix_attention",
+         [](const Tensor&, const Tensor&, const Tensor&, const optional<Tensor>&, const Tensor&,
+            const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+            const Tensor&, const Tensor&, bool, optional<double>) -> Tensor {
+           host_tensors("shared_prefix_attention");
          });
 }

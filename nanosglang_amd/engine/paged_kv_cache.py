@@ -37,6 +37,8 @@ from dataclasses import dataclass, field
 
 import torch
 
+from .. import kernels
+
 
 @dataclass
 class BlockTable:
@@ -49,7 +51,12 @@ class BlockTable:
 
 
 class BlockManager:
-    """Pool of fixed-size KV blocks shared by all layers (:35-171)."""
+    """Pool of fixed-size KV blocks shared by all layers (:35-171).
+
+    With ``dtype=torch.float8_e4m3fn`` the caches hold e4m3 codes and
+    ``kv_scale`` (num_layers, num_blocks, num_kv_heads, 2, block_size) uint8 the
+    scale of each row (``kernels.kv_write_fp8``); ``write_kv`` / ``read_kv`` then
+    take and give bf16 rows, on the GPU.  Otherwise ``kv_scale`` is None."""
 
     def __init__(self, num_blocks: int, block_size: int, num_layers: int, num_kv_heads: int,
                  head_dim: int, dtype: torch.dtype = torch.float16, device: str = "cuda"):
@@ -63,8 +70,20 @@ class BlockManager:
         shape = (num_layers, num_blocks, block_size, num_kv_heads, head_dim)
         self.k_cache = torch.zeros(shape, dtype=dtype, device=device)
         self.v_cache = torch.zeros(shape, dtype=dtype, device=device)
+        self.kv_scale = None
+        if dtype == torch.float8_e4m3fn:
+            self.kv_scale = torch.zeros(num_layers, num_blocks, num_kv_heads, 2, block_size,
+                                        dtype=torch.uint8, device=device)
         self.free_blocks: list[int] = list(range(num_blocks))
         self.ref_counts: dict[int, int] = {}
+
+    @property
+    def caches(self) -> tuple[torch.Tensor, ...]:
+        """(k_cache, v_cache), with kv_scale for the 8-bit pool: the
+        ``kv_cache`` of ``CausalLM.forward_packed``."""
+        if self.kv_scale is None:
+            return self.k_cache, self.v_cache
+        return self.k_cache, self.v_cache, self.kv_scale
 
     @property
     def num_free_blocks(self) -> int:
@@ -110,6 +129,15 @@ class BlockManager:
                  v: torch.Tensor) -> None:
         """k, v: (num_kv_heads, num_tokens, head_dim) -> NHD rows (:122-137)."""
         n = k.shape[1]
+        if self.kv_scale is not None:
+            if not 0 <= slot_offset <= self.block_size - n:
+                raise ValueError(f"{n} tokens at offset {slot_offset} do not fit a block of "
+                                 f"{self.block_size}")
+            slots = torch.arange(n, device=self.k_cache.device) + (block_id * self.block_size
+                                                                  + slot_offset)
+            kernels.kv_write_fp8(k.transpose(0, 1).contiguous(), v.transpose(0, 1).contiguous(),
+                                 slots, *(t[layer_idx] for t in self.caches))
+            return
         self.k_cache[layer_idx, block_id, slot_offset:slot_offset + n] = k.transpose(0, 1)
         self.v_cache[layer_idx, block_id, slot_offset:slot_offset + n] = v.transpose(0, 1)
 
@@ -118,13 +146,18 @@ class BlockManager:
         P = self.block_size
         need = (total_tokens + P - 1) // P
         idx = torch.as_tensor(block_ids[:need], device=self.k_cache.device)
+        if self.kv_scale is not None:
+            slots = (idx.long()[:, None] * P + torch.arange(P, device=idx.device)).reshape(-1)
+            k, v = kernels.kv_read_fp8(slots[:total_tokens],
+                                       *(t[layer_idx] for t in self.caches))
+            return k.transpose(0, 1), v.transpose(0, 1)
         k = self.k_cache[layer_idx, idx].reshape(-1, self.num_kv_heads, self.head_dim)
         v = self.v_cache[layer_idx, idx].reshape(-1, self.num_kv_heads, self.head_dim)
         return k[:total_tokens].transpose(0, 1), v[:total_tokens].transpose(0, 1)
 
     @property
     def memory_bytes(self) -> int:
-        return (self.k_cache.nelement() + self.v_cache.nelement()) * self.k_cache.element_size()
+        return sum(t.nelement() * t.element_size() for t in self.caches)
 
     def __repr__(self) -> str:
         used = self.num_blocks - self.num_free_blocks

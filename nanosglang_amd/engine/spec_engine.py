@@ -205,7 +205,8 @@ class SpecEngine:
                  block_size: int = 16, temperature: float = 0.0, seed: int = 0,
                  workspace_bytes: int = 256 << 20, use_graphs: bool = True,
                  max_batch: int = 32, top_k: int = 0, top_p: float = 1.0,
-                 kv_split: bool = False, pipeline: bool = True):
+                 kv_split: bool = False, pipeline: bool = True,
+                 kv_dtype: torch.dtype = torch.bfloat16):
         c = model.config
         self.model = model
         self.k = num_speculative
@@ -220,7 +221,7 @@ class SpecEngine:
         self.seed = seed
         self.device = model.device
         self.bm = BlockManager(num_blocks, block_size, model.num_layers, c.num_key_value_heads,
-                               c.head_dim, dtype=torch.bfloat16, device=self.device)
+                               c.head_dim, dtype=kernels._kv_dtype(kv_dtype), device=self.device)
         self.kv = PagedKVCache(self.bm)
         self.P = block_size
         self.attn_ws = torch.empty(workspace_bytes, dtype=torch.uint8, device=self.device)
@@ -278,7 +279,7 @@ class SpecEngine:
             last[i] = L - (npg - 1) * P
         idx = np.asarray(idx, np.int32)
         self.attn.plan(qo, kvp, idx, last, c.num_attention_heads, c.num_key_value_heads,
-                       c.head_dim, P, causal=True)
+                       c.head_dim, P, causal=True, kv_data_type=self.bm.dtype)
         return kvp, idx
 
     def _slots(self, reqs, starts, counts) -> np.ndarray:
@@ -299,7 +300,7 @@ class SpecEngine:
             t.to(self.device, dtype, non_blocking=False)
 
     def _pool(self):
-        return (self.bm.k_cache, self.bm.v_cache)
+        return self.bm.caches
 
     def _sample_rows(self, logits: torch.Tensor) -> torch.Tensor:
         """One token per row: argmax if greedy, else inverse CDF of
@@ -382,7 +383,8 @@ class SpecEngine:
             for a, w in enumerate(g.attn):
                 ql = 1 if a < self.k else self.k + 1
                 w.adopt_plan(g.plans[a], bs * ql, c.num_attention_heads,
-                             c.num_key_value_heads, c.head_dim, self.P, causal=True)
+                             c.num_key_value_heads, c.head_dim, self.P, causal=True,
+                             kv_data_type=self.bm.dtype)
             g.arena.upload()
             for _ in range(2):                           # warm-up (allocator, GEMM heuristics)
                 self._graph_body(g)
@@ -728,6 +730,21 @@ class SpecEngine:
                          rollback, None, dlog, u)
         return n_out.cpu().numpy(), emitted.cpu().numpy()
 
+    def _fill_noise(self, g: torch.Generator) -> None:
+        """Normal K / V rows in every slot of the pool."""
+        bm = self.bm
+        if bm.kv_scale is None:
+            for pool in self._pool():
+                for layer in pool:
+                    layer.normal_(generator=g)
+            return
+        slots = torch.arange(bm.num_blocks * self.P, device=self.device)
+        for li in range(bm.num_layers):
+            for part in slots.split(65536):
+                k, v = (torch.randn(len(part), bm.num_kv_heads, bm.head_dim, generator=g,
+                                    device=self.device, dtype=torch.bfloat16) for _ in range(2))
+                kernels.kv_write_fp8(k, v, part, *(t[li] for t in self._pool()))
+
     # ---- main entry ----
     def _admit(self, reqs: list, synthetic_context: bool = False) -> None:
         """Admission and prefill: a block table per request
@@ -746,9 +763,7 @@ class SpecEngine:
         if synthetic_context:
             if not self._noise:
                 g = torch.Generator(device=self.device).manual_seed(self.seed)
-                for pool in self._pool():
-                    for layer in pool:
-                        layer.normal_(generator=g)
+                self._fill_noise(g)
                 self._noise = True
             first = [r.prompt[-1] for r in reqs]
         else:

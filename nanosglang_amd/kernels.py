@@ -880,6 +880,13 @@ def sample(logits: torch.Tensor, temperature: float, top_k: int = 0, top_p: floa
     return out
 
 
+def _refuse_fp8_pool(k_cache, v_cache, use: str) -> None:
+    """An 8-bit pool has half the bytes that a bf16 kernel writes."""
+    if (k_cache is not None and k_cache.dtype == FP8) or \
+            (v_cache is not None and v_cache.dtype == FP8):
+        raise TypeError(f"the caches are an 8-bit pool: {use}")
+
+
 def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: torch.Tensor,
              v_cache: torch.Tensor) -> None:
     """k, v: (T, Hkv, D) bf16 (rows may be strided views); slots int64 (T,);
@@ -894,6 +901,7 @@ def kv_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: tor
         raise ValueError("each K/V row must be a contiguous (Hkv, D) block")
     if k_cache.dtype != torch.bfloat16 or k.dtype != torch.bfloat16:
         raise TypeError("K/V and caches must be bfloat16")
+    _refuse_fp8_pool(k_cache, v_cache, "use kv_write_fp8")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("caches must be contiguous")
     if k_cache.shape[-2:] != (Hkv, D):
@@ -999,6 +1007,7 @@ def kv_read_fp8(slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 def kv_clear_slots(slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
     """Zero flat slots in every layer of (L, N, P, Hkv, D) pools."""
     _require_gpu(slots, "slots")
+    _refuse_fp8_pool(k_cache, v_cache, "its rows are not cleared, only written again")
     L, N, P, Hkv, D = k_cache.shape
     slots = slots.reshape(-1).to(torch.int64).contiguous()
     check(_lib().nsg_kv_clear_slots(slots.data_ptr(), slots.numel(), k_cache.data_ptr(),
@@ -1019,6 +1028,7 @@ def rope_kv_write(qkv: torch.Tensor, num_qo_heads: int, num_kv_heads: int, head_
     T = qkv.shape[0]
     if qkv.dtype != torch.bfloat16 or qkv.stride(-1) != 1:
         raise ValueError("qkv must be bfloat16 with unit inner stride")
+    _refuse_fp8_pool(k_cache, v_cache, "use rope_kv_write_fp8")
     if q_out is None:
         q_out = torch.empty(T, num_qo_heads, head_dim, dtype=torch.bfloat16, device=qkv.device)
     positions = positions.to(torch.int64).contiguous()
@@ -1427,6 +1437,22 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     return out
 
 
+_ROW_IDS: dict = {}
+
+
+def _row_ids(device: torch.device, n: int) -> torch.Tensor:
+    """int64 0 .. n - 1 on ``device``, kept from call to call (a tensor made while
+    a graph is captured holds nothing before its replay, and is not kept)."""
+    t = _ROW_IDS.get(device)
+    if t is None or t.numel() < n:
+        t = torch.arange(max(n, _lib().nsg_linear_max_rows()), device=device)
+        if torch.cuda.is_current_stream_capturing():
+            return t[:n]
+        torch.cuda.current_stream(device).synchronize()      # for other streams' use
+        _ROW_IDS[device] = t
+    return t[:n]
+
+
 def linear_rope_kv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None,
                    num_qo_heads: int, num_kv_heads: int, head_dim: int,
                    positions: torch.Tensor, cos_table: torch.Tensor, sin_table: torch.Tensor,
@@ -1435,7 +1461,8 @@ def linear_rope_kv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
                    force: bool = False, w_scale: torch.Tensor | None = None,
                    w_dequant: torch.Tensor | None = None,
                    sumsq_in: torch.Tensor | None = None,
-                   norm_eps: float = 1e-6) -> torch.Tensor:
+                   norm_eps: float = 1e-6,
+                   kv_scale: torch.Tensor | None = None) -> torch.Tensor:
     """q/k/v projection + RoPE + KV-slot write (C ABI: nsg_linear_rope_kv, or
     nsg_linear_rope_kv_fp8 for float8_e4m3fn weights with per-row w_scale).
 
@@ -1445,11 +1472,18 @@ def linear_rope_kv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     faster projection (prefill), or for shapes the fused kernel does not take,
     it runs exactly that pair.
     ``sumsq_in``: the folded RMSNorm's consumer side (nsg_linear_rope_kv_fold,
-    see ``linear``; the fused kernel only).  Returns rotated q (M, Hq, D)."""
+    see ``linear``; the fused kernel only).  With ``kv_scale`` the caches are an
+    8-bit pool: the pair is then ``rope_kv_write_fp8(linear(...), ...)``, and the
+    fused kernel, whose tiles hold parts of a row, writes bf16 rows that
+    ``kv_write_fp8`` quantises.  Returns rotated q (M, Hq, D)."""
     _require_gpu(x, "x")
     M, K = x.shape
     lib = _lib()
     N = weight.shape[0]
+    if kv_scale is None:
+        _refuse_fp8_pool(k_cache, v_cache, "it needs its kv_scale")
+    elif slots is None:
+        raise ValueError("kv_scale without slots to write")
     fp8 = _check_fp8(weight, w_scale, K)
     if sumsq_in is not None and (fp8 or M > lib.nsg_linear_max_rows()):
         raise ValueError("the folded RMSNorm takes bf16 weights and at most "
@@ -1462,6 +1496,10 @@ def linear_rope_kv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     if not fits or not (force or fp8 or sumsq_in is not None
                         or lib.nsg_linear_preferred(M, N, K)):
         qkv = linear(x, weight, bias, w_scale=w_scale, w_dequant=w_dequant)
+        if kv_scale is not None:
+            return rope_kv_write_fp8(qkv, num_qo_heads, num_kv_heads, head_dim, positions,
+                                     cos_table, sin_table, slots, k_cache, v_cache, kv_scale,
+                                     q_out)
         return rope_kv_write(qkv, num_qo_heads, num_kv_heads, head_dim, positions, cos_table,
                              sin_table, slots, k_cache, v_cache, q_out)
     if not fp8 and (weight.dtype != torch.bfloat16 or weight.stride(1) != 1
@@ -1469,6 +1507,14 @@ def linear_rope_kv(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
         raise ValueError("weight must be bf16 (N, K) with unit inner stride")
     if bias is not None and (bias.dtype != torch.bfloat16 or not bias.is_contiguous()):
         raise ValueError("bias must be contiguous bf16")
+    if kv_scale is not None:
+        _check_fp8_pool(k_cache, v_cache, kv_scale, num_kv_heads, head_dim, x.device)
+        kv = torch.empty(2, 1, M, num_kv_heads, head_dim, dtype=torch.bfloat16, device=x.device)
+        q_out = linear_rope_kv(x, weight, bias, num_qo_heads, num_kv_heads, head_dim, positions,
+                               cos_table, sin_table, _row_ids(x.device, M), kv[0], kv[1], q_out,
+                               True, w_scale, w_dequant, sumsq_in, norm_eps)
+        kv_write_fp8(kv[0, 0], kv[1, 0], slots, k_cache, v_cache, kv_scale)
+        return q_out
     if q_out is None:
         q_out = torch.empty(M, num_qo_heads, head_dim, dtype=torch.bfloat16, device=x.device)
     positions = positions.to(torch.int64).contiguous()

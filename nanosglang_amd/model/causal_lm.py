@@ -213,6 +213,19 @@ class CausalLM:
     def num_layers(self) -> int:
         return self.config.num_hidden_layers
 
+    def _attention(self, x, weight, bias, positions, slots, cache, attn_wrapper, **linear_args):
+        """One layer's q/k/v projection of rows x, RoPE, KV write and paged
+        attention (T, Hq, D); cache: its (k_cache, v_cache), with kv_scale
+        where the pool is 8-bit."""
+        c = self.config
+        kv_scale = cache[2] if len(cache) == 3 else None
+        q = kernels.linear_rope_kv(x, weight, bias, c.num_attention_heads, c.num_key_value_heads,
+                                   c.head_dim, positions, self.rope_cos, self.rope_sin, slots,
+                                   *cache[:2], kv_scale=kv_scale, **linear_args)
+        if kv_scale is None:
+            return attn_wrapper.run(q, cache)
+        return attn_wrapper.run(q, cache[:2], kv_scale=kv_scale)
+
     @torch.inference_mode()
     def forward_packed(self, input_ids: torch.Tensor, positions: torch.Tensor, kv_cache,
                        attn_wrapper, write_indices: torch.Tensor,
@@ -223,8 +236,10 @@ class CausalLM:
                        ids_keys: tuple | None = None):
         """Packed forward over ``T`` tokens of several requests.
 
-        kv_cache: (k_cache, v_cache) pools (L, N, P, Hkv, D); attn_wrapper: a
-        planned ``BatchPrefillWithPagedKVCacheWrapper``; write_indices: int64
+        kv_cache: (k_cache, v_cache) pools (L, N, P, Hkv, D), or (k_cache,
+        v_cache, kv_scale) of the 8-bit pool, kv_scale (L, N, Hkv, 2, P) uint8;
+        attn_wrapper: a ``BatchPrefillWithPagedKVCacheWrapper`` or
+        ``SharedPrefixAttentionWrapper`` planned for that pool; write_indices: int64
         flat slots (T,).  Returns logits (len(logit_indices) or T, V), or,
         with ``argmax_out`` (int64, one per row), each row's greedy token
         written there (``kernels.linear_argmax``: the logits are never
@@ -237,9 +252,7 @@ class CausalLM:
         those greedy tokens inside the embedding lookup -- no reduction
         launch between the two forwards.  Both need ``keys_supported``."""
         c = self.config
-        Hq, Hkv, D, I = (c.num_attention_heads, c.num_key_value_heads, c.head_dim,
-                         c.intermediate_size)
-        k_pool, v_pool = kv_cache
+        Hq, D = c.num_attention_heads, c.head_dim
         nl = self.num_layers if num_layers is None else num_layers
         eps = c.rms_norm_eps
         T = input_ids.numel()
@@ -270,11 +283,9 @@ class CausalLM:
             ssb = torch.empty_like(ssa)
             for li in range(nl):
                 L = self.layers[li]
-                q = kernels.linear_rope_kv(residual, L["qkv_g"], L["qkv_b"], Hq, Hkv, D,
-                                           positions, self.rope_cos, self.rope_sin,
-                                           write_indices, k_pool[li], v_pool[li],
-                                           sumsq_in=ssa, norm_eps=eps)
-                attn = attn_wrapper.run(q, (k_pool[li], v_pool[li]))
+                attn = self._attention(residual, L["qkv_g"], L["qkv_b"], positions,
+                                       write_indices, [t[li] for t in kv_cache], attn_wrapper,
+                                       sumsq_in=ssa, norm_eps=eps)
                 kernels.linear(attn.view(-1, Hq * D), L["o"], residual=residual, sumsq_out=ssb)
                 g = kernels.linear(residual, L["gate_up_g"], swiglu=True, sumsq_in=ssb,
                                    norm_eps=eps)
@@ -308,11 +319,9 @@ class CausalLM:
                 # residual += x (causal_lm.py:505, 531), then RMSNorm -- one kernel
                 h = kernels.rmsnorm(residual if x is None else x, ln1, eps,
                                     residual=None if x is None else residual)
-                q = kernels.linear_rope_kv(h, L[qkv_k], L["qkv_b"], Hq, Hkv, D, positions,
-                                           self.rope_cos, self.rope_sin, write_indices,
-                                           k_pool[li], v_pool[li], w_scale=L.get("qkv_s"),
-                                           w_dequant=L.get("qkv_d"))
-                attn = attn_wrapper.run(q, (k_pool[li], v_pool[li]))
+                attn = self._attention(h, L[qkv_k], L["qkv_b"], positions, write_indices,
+                                       [t[li] for t in kv_cache], attn_wrapper,
+                                       w_scale=L.get("qkv_s"), w_dequant=L.get("qkv_d"))
                 x = kernels.linear(attn.view(-1, Hq * D), L["o"], w_scale=L.get("o_s"),
                                    w_dequant=L.get("o_d"))
                 h = kernels.rmsnorm(x, ln2, eps, residual=residual)   # causal_lm.py:147-154

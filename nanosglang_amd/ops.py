@@ -29,6 +29,15 @@ nano_sglang/model/causal_lm.py:340), the KV ``index_put`` (causal_lm.py:
     temperature / top-k / top-p sampling, one token per row.
 ``nsg::kv_write``, ``nsg::rope_kv_write``
     K/V rows (after RoPE, for the second) into their flat KV slots.
+``nsg::kv_write_fp8``, ``nsg::rope_kv_write_fp8``, ``nsg::kv_read_fp8``
+    the same into the 8-bit pool (``kernels.kv_write_fp8``), and rows of it as
+    bf16.
+``nsg::verify_attention_fp8``, ``nsg::verify_attention_run_fp8``
+    attention over the 8-bit pool, planned by ``nsg::verify_attention_plan``.
+``nsg::shared_prefix_attention``
+    plan + run of ``kernels.SharedPrefixAttentionWrapper`` (either pool:
+    ``kv_scale`` None is bf16); it synchronises as ``nsg::verify_attention``
+    does.
 
 This module loads the operator library and registers the shape-only (fake)
 implementations that tracing and compilation use.
@@ -128,6 +137,43 @@ def _(k, v, slots, k_cache, v_cache):
 def _(qkv, num_qo_heads, num_kv_heads, head_dim, positions, cos_table, sin_table, slots,
       k_cache, v_cache):
     return qkv.new_empty((qkv.shape[0], num_qo_heads, head_dim))
+
+
+@torch.library.register_fake("nsg::kv_write_fp8")
+def _(k, v, slots, k_cache, v_cache, kv_scale):
+    return None
+
+
+@torch.library.register_fake("nsg::kv_read_fp8")
+def _(slots, k_cache, v_cache, kv_scale):
+    shape = (slots.numel(), k_cache.shape[2], k_cache.shape[3])
+    return (k_cache.new_empty(shape, dtype=torch.bfloat16),
+            k_cache.new_empty(shape, dtype=torch.bfloat16))
+
+
+@torch.library.register_fake("nsg::rope_kv_write_fp8")
+def _(qkv, num_qo_heads, num_kv_heads, head_dim, positions, cos_table, sin_table, slots,
+      k_cache, v_cache, kv_scale):
+    return qkv.new_empty((qkv.shape[0], num_qo_heads, head_dim))
+
+
+@torch.library.register_fake("nsg::verify_attention_fp8")
+def _(q, k_cache, v_cache, kv_scale, qo_indptr, paged_kv_indptr, paged_kv_indices,
+      paged_kv_last_page_len, causal=True, sm_scale=None):
+    return torch.empty_like(q)
+
+
+@torch.library.register_fake("nsg::verify_attention_run_fp8")
+def _(plan, work, q, k_cache, v_cache, kv_scale, paged_kv_indices, sm_scale, causal, workspace,
+      out):
+    return None
+
+
+@torch.library.register_fake("nsg::shared_prefix_attention")
+def _(q, k_cache, v_cache, kv_scale, qo_indptr, group_indptr, prefix_kv_indptr,
+      prefix_kv_indices, prefix_kv_last_page_len, paged_kv_indptr, paged_kv_indices,
+      paged_kv_last_page_len, causal=True, sm_scale=None):
+    return torch.empty_like(q)
 
 
 __all__ = ["plan_record", "plan_from_record", "plan_workspace_bytes", "RECORD_INTS", "LIB_PATH"]

@@ -1,0 +1,125 @@
+"""The 8-bit pool's and the shared prefix's torch operators, and the 8-bit
+pool's users, on a host without a GPU: schemas, shapes, refusals."""
+import numpy as np
+import pytest
+import torch
+
+from nanosglang_amd import kernels, ops  # noqa: F401  (ops loads the operators)
+from nanosglang_amd.engine.paged_kv_cache import BlockManager, PagedKVCache
+
+FP8 = torch.float8_e4m3fn
+POOL = ["k_cache", "v_cache", "kv_scale"]
+PAGES = ["paged_kv_indptr", "paged_kv_indices", "paged_kv_last_page_len"]
+
+
+@pytest.mark.parametrize("name,args,written", [
+    ("kv_write_fp8", ["k", "v", "slots"] + POOL, set(POOL)),
+    ("kv_read_fp8", ["slots"] + POOL, set()),
+    ("rope_kv_write_fp8", ["qkv", "num_qo_heads", "num_kv_heads", "head_dim", "positions",
+                           "cos_table", "sin_table", "slots"] + POOL, set(POOL)),
+    ("verify_attention_fp8", ["q"] + POOL + ["qo_indptr"] + PAGES + ["causal", "sm_scale"], set()),
+    ("verify_attention_run_fp8", ["plan", "work", "q"] + POOL + [
+        "paged_kv_indices", "sm_scale", "causal", "workspace", "out"], {"workspace", "out"}),
+    ("shared_prefix_attention", ["q"] + POOL + [
+        "qo_indptr", "group_indptr", "prefix_kv_indptr", "prefix_kv_indices",
+        "prefix_kv_last_page_len"] + PAGES + ["causal", "sm_scale"], set()),
+])
+def test_schemas_and_kernels(name, args, written):
+    schema = getattr(torch.ops.nsg, name).default._schema
+    assert [a.name for a in schema.arguments] == args
+    assert {a.name for a in schema.arguments
+            if a.alias_info is not None and a.alias_info.is_write} == written
+    for key in ("CUDA", "CPU"):
+        assert torch._C._dispatch_has_kernel_for_dispatch_key(f"nsg::{name}", key), key
+
+
+def _args(device):
+    i32 = dict(dtype=torch.int32, device=device)
+    pool = [torch.empty(8, 16, 2, 64, device=device, dtype=FP8) for _ in range(2)]
+    pool.append(torch.empty(8, 2, 2, 16, device=device, dtype=torch.uint8))
+    csr = [torch.empty(3, **i32), torch.empty(5, **i32), torch.empty(2, **i32)]
+    row = lambda *s: torch.empty(*s, device=device, dtype=torch.bfloat16)
+    slots = torch.empty(6, device=device, dtype=torch.int64)
+    tab = torch.empty(64, 32, device=device)
+    qo = torch.empty(3, **i32)
+    return dict(
+        kv_write_fp8=[row(6, 2, 64), row(6, 2, 64), slots, *pool],
+        kv_read_fp8=[slots, *pool],
+        rope_kv_write_fp8=[row(6, 18 * 64), 14, 2, 64, slots, tab, tab, slots, *pool],
+        verify_attention_fp8=[row(6, 14, 64), *pool, qo, *csr],
+        verify_attention_run_fp8=[qo, qo, row(6, 14, 64), *pool, csr[1], 0.125, True, slots,
+                                  row(6, 14, 64)],
+        shared_prefix_attention=[row(6, 14, 64), *pool, qo, torch.empty(2, **i32),
+                                 torch.empty(2, **i32), torch.empty(4, **i32),
+                                 torch.empty(1, **i32), *csr])
+
+
+def test_shapes_without_a_gpu():
+    a = _args("meta")
+    op = torch.ops.nsg
+    for x in op.kv_read_fp8(*a["kv_read_fp8"]):
+        assert (x.shape, x.dtype) == ((6, 2, 64), torch.bfloat16)
+    for name in ("rope_kv_write_fp8", "verify_attention_fp8", "shared_prefix_attention"):
+        x = getattr(op, name)(*a[name])
+        assert (x.shape, x.dtype) == ((6, 14, 64), torch.bfloat16), name
+    assert op.kv_write_fp8(*a["kv_write_fp8"]) is None
+
+
+@pytest.mark.parametrize("name", list(_args("meta")))
+def test_operators_refuse_host_tensors(name):
+    with pytest.raises(RuntimeError, match="GPU tensor"):
+        getattr(torch.ops.nsg, name)(*_args("cpu")[name])
+
+
+def test_block_manager_of_an_8_bit_pool():
+    bm = BlockManager(6, 16, 3, 2, 64, FP8, "cpu")
+    assert [t.dtype for t in bm.caches] == [FP8, FP8, torch.uint8]
+    assert bm.kv_scale.shape == (3, 6, 2, 2, 16)
+    assert bm.memory_bytes == 3 * 6 * 16 * 2 * (2 * 64 + 2)
+    t = PagedKVCache(bm).allocate_for_request(40)
+    z = torch.zeros(2, 5, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="GPU tensor"):        # no CPU path
+        bm.write_kv(t.block_indices[0], 0, 3, z, z)
+    with pytest.raises(ValueError, match="do not fit"):          # the next block's slots
+        bm.write_kv(t.block_indices[0], 0, 12, z, z)
+    plain = BlockManager(6, 16, 3, 2, 64, torch.bfloat16, "cpu")
+    assert plain.kv_scale is None and len(plain.caches) == 2
+
+
+def test_bf16_writers_refuse_the_8_bit_pool(monkeypatch):
+    """They would write two bytes for each of the pool's one."""
+    monkeypatch.setattr(kernels, "_require_gpu", lambda *a: None)
+    pool = torch.zeros(4, 16, 2, 64, dtype=FP8)
+    bf = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    z = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    x, w = torch.zeros(3, 64, dtype=torch.bfloat16), torch.zeros(256, 64, dtype=torch.bfloat16)
+    s = torch.zeros(3, dtype=torch.int64)
+    for k, v in ((pool, pool), (bf, pool), (pool, bf)):
+        with pytest.raises(TypeError):
+            kernels.kv_write(z, z, s, k, v)
+        with pytest.raises(TypeError, match="8-bit pool"):
+            kernels.rope_kv_write(torch.zeros(3, 512, dtype=torch.bfloat16), 4, 2, 64, s, s, s, s,
+                                  k, v)
+        with pytest.raises(TypeError, match="8-bit pool"):
+            kernels.linear_rope_kv(x, w, None, 0, 2, 64, s, s, s, s, k, v)
+        with pytest.raises(TypeError, match="8-bit pool"):
+            kernels.kv_clear_slots(s, k[None], v[None])
+
+
+def test_projection_into_the_8_bit_pool_refuses(monkeypatch):
+    monkeypatch.setattr(kernels, "_require_gpu", lambda *a: None)
+    x, w = torch.zeros(3, 64, dtype=torch.bfloat16), torch.zeros(512, 64, dtype=torch.bfloat16)
+    s, tab = torch.zeros(3, dtype=torch.int64), torch.zeros(8, 32)
+    pool = torch.zeros(4, 16, 2, 64, dtype=FP8)
+    sc = torch.zeros(4, 2, 2, 16, dtype=torch.uint8)
+    bf = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    call = lambda *a, **kw: kernels.linear_rope_kv(x, w, None, 4, 2, 64, s, tab, tab, *a,
+                                                   force=True, **kw)
+    with pytest.raises(TypeError, match="float8_e4m3fn"):
+        call(s, bf, bf, kv_scale=sc)
+    with pytest.raises(ValueError, match="kv_scale must be"):
+        call(s, pool, pool, kv_scale=sc[1:])
+    with pytest.raises(ValueError, match="do not match"):
+        call(s, pool[:, :, :1].contiguous(), pool[:, :, :1].contiguous(), kv_scale=sc)
+    with pytest.raises(ValueError, match="without slots"):
+        call(None, None, None, kv_scale=sc)
