@@ -227,9 +227,11 @@ def test_engine_over_the_8_bit_pool(graphs):
     eng.trace = []
     held = []
     free = eng.kv.free_request
-    eng.kv.free_request = lambda t: (held.append((list(t.block_indices), _values(eng.bm, 0))),
+    bm = eng.bm
+    eng.kv.free_request = lambda t: (held.append((list(t.block_indices), _values(bm, 0))),
                                      free(t))
     out = eng.generate(prompts, max_new)
+    del eng.kv.free_request              # (no cycle that keeps the engine's graphs alive)
     assert [len(o) for o in out] == max_new
     assert eng.bm.num_free_blocks == 64 - graphs
     assert eng.trace
