@@ -106,12 +106,14 @@ __global__ __launch_bounds__(RT * KS * 64) void verify_attn_fp8_kernel(AttnParam
 
   int wi = blockIdx.y;
   int h = blockIdx.x;
-  if constexpr (D == 64) {
+  if constexpr (D == 64 && KS == 1) {
     // Two heads' rows of 64 bytes share a cache line: workgroups L and L + 8,
     // which the round-robin puts on one XCD, take the two heads of a pair, so
     // that a line comes to one L2 instead of two.  40 requests x 2 rows over
     // 1000 - 5000 tokens, 16 heads of 64: 97 us without, 76.5 with; 64 x 5 rows over
-    // 1000 - 8192, 2 KV heads: 43 and 36.  Blocks of 16, the last as wide as it is.
+    // 1000 - 8192, 2 KV heads: 43 and 36.  Several KV groups, short contexts: 5.0 us
+    // without, 5.2 with (one request of 350 tokens).  Blocks of 16, the last as
+    // wide as it is.
     if ((p.Hkv & 1) == 0) {
       const uint32_t n = gridDim.x * gridDim.y, l = blockIdx.y * gridDim.x + blockIdx.x;
       const uint32_t b0 = l & ~15u, half = min(16u, n - b0) / 2, at = l - b0;
