@@ -18,7 +18,8 @@
 // pass over K and goes through its steps once more.  Dropping the running maximum
 // (16 max3, a swap, 64 multiplies or, around a branch, as many register moves of
 // the accumulators per step) measured at 4 x 1000-token chunks over 2048 - 8192,
-// 32 / 8 heads of 128, from 413 to 386 us (0.74 PFLOP/s of the causal products).
+// 32 / 8 heads of 128, a kernel alone, from 413 to 386 us (pass after pass 326 us,
+// 0.87 PFLOP/s of the causal products).
 #pragma once
 
 #include "attention.hpp"

@@ -435,7 +435,9 @@ class SharedPrefixAttentionWrapper:
     graph captured around ``run`` replays after each re-plan (``max_kv_len`` > 0
     bounds a request's own tokens, and then they are never split); a plan of
     fewer query rows leaves the rest of ``out`` as it was.  Without it a captured
-    ``run`` keeps the plan it was captured with."""
+    ``run`` keeps the plan it was captured with.  The workspace holds partial
+    rows between the kernels of a ``run``: runs (and replays) that may overlap on
+    two streams need wrappers and workspaces of their own."""
 
     def __init__(self, float_workspace_buffer: torch.Tensor, kv_layout: str = "NHD",
                  num_cus: int = MI355X_CUS, use_cuda_graph: bool = False,
@@ -512,6 +514,7 @@ class SharedPrefixAttentionWrapper:
             self._work, self._idx = (
                 torch.from_numpy(x if len(x) else np.zeros(1, np.int32)).to(self._device)
                 for x in (work, ids))
+            self._streams = {torch._C._cuda_getCurrentRawStream(self._device.index)}
         self._plan = pl
         self._kv_dtype = kv_dtype
         self._total_q = int(qo[-1])
@@ -589,8 +592,15 @@ class SharedPrefixAttentionWrapper:
             raise ValueError(f"out must be contiguous bfloat16 {tuple(q.shape)}")
         _same_device(self._device, q=q, k_cache=k_cache, v_cache=v_cache, kv_scale=kv_scale,
                      out=out)
-        if not self._graph and torch.cuda.is_current_stream_capturing():
-            self._captured.append((self._work, self._idx))
+        if not self._graph:
+            if torch.cuda.is_current_stream_capturing():
+                self._captured.append((self._work, self._idx))
+            elif torch._C._cuda_getCurrentRawStream(self._device.index) not in self._streams:
+                # the next plan frees these while this stream may still read them
+                stream = torch.cuda.current_stream(self._device)
+                self._streams.add(stream.cuda_stream)
+                self._work.record_stream(stream)
+                self._idx.record_stream(stream)
         _launch(self._device, _lib().nsg_prefix_attn_run, "nsg_prefix_attn_run",
                 C.byref(self._plan), self._work.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
                 v_cache.data_ptr(), _ptr(kv_scale), out.data_ptr(), self._idx.data_ptr(),

@@ -231,6 +231,33 @@ def test_graph_mode_replays_after_each_plan(fp8, max_kv_len, Hq):
         assert (out[n:] == 9.0).all()
 
 
+def test_a_run_on_another_stream_outlives_the_next_plan():
+    """The plan's arrays go back to the allocator when the wrapper plans again,
+    but not while another stream's run may still read them."""
+    rng = np.random.default_rng(8)
+    heads, P = (14, 2, 64), 16
+    caches, sc, k, v = _pool(rng, True, 300, P, 2, 64)
+    w = _wrapper()
+    c = dict(q=[2] * 8, kv=[20] * 8, groups=[0, 8], prefix=[2000])
+    ptabs, tabs = _tables(rng, c, P, 300)
+    q = fc.bf16(rng.standard_normal((16, 14, 64)))
+    qd = torch.from_numpy(q).cuda().bfloat16()
+    side = torch.cuda.Stream()
+    want = _want(q, c, ptabs, tabs, k, v)
+    for _ in range(3):
+        _plan(w, c, ptabs, tabs, heads, P, True)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)                # about 10 ms before the run starts
+            out = w.run(qd, caches, kv_scale=sc)
+        c2 = dict(q=[1], kv=[7], groups=[0, 1], prefix=[100])
+        _plan(w, c2, *_tables(rng, c2, P, 300), heads, P, True)
+        junk = [torch.zeros(n, dtype=torch.int32, device="cuda") for n in (64, 200, 500, 1000) * 8]
+        torch.cuda.synchronize()
+        del junk
+        fc.check(out, *want)
+
+
 def test_a_captured_run_keeps_its_plan():
     """Without graph mode: a later plan leaves the captured graph's arrays
     alone, and a wrapper plans and runs on."""
