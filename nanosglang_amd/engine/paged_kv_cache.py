@@ -53,13 +53,15 @@ class BlockTable:
 class BlockManager:
     """Pool of fixed-size KV blocks shared by all layers (:35-171).
 
-    With ``dtype=torch.float8_e4m3fn`` the caches hold e4m3 codes and
-    ``kv_scale`` (num_layers, num_blocks, num_kv_heads, 2, block_size) uint8 the
-    scale of each row (``kernels.kv_write_fp8``); ``write_kv`` / ``read_kv`` then
-    take and give bf16 rows, on the GPU.  Otherwise ``kv_scale`` is None."""
+    With ``row_scales`` (``dtype=torch.float8_e4m3fn``) the caches hold e4m3
+    codes and ``kv_scale`` (num_layers, num_blocks, num_kv_heads, 2, block_size)
+    uint8 the scale of each row (``kernels.kv_write_fp8``); ``write_kv`` /
+    ``read_kv`` then take and give bf16 rows, on the GPU.  Otherwise
+    ``kv_scale`` is None."""
 
     def __init__(self, num_blocks: int, block_size: int, num_layers: int, num_kv_heads: int,
-                 head_dim: int, dtype: torch.dtype = torch.float16, device: str = "cuda"):
+                 head_dim: int, dtype: torch.dtype = torch.float16, device: str = "cuda",
+                 row_scales: bool = False):
         self.num_blocks = num_blocks
         self.block_size = block_size
         self.num_layers = num_layers
@@ -71,7 +73,9 @@ class BlockManager:
         self.k_cache = torch.zeros(shape, dtype=dtype, device=device)
         self.v_cache = torch.zeros(shape, dtype=dtype, device=device)
         self.kv_scale = None
-        if dtype == torch.float8_e4m3fn:
+        if row_scales:
+            if dtype != torch.float8_e4m3fn:
+                raise ValueError(f"row_scales is for float8_e4m3fn caches, not {dtype}")
             self.kv_scale = torch.zeros(num_layers, num_blocks, num_kv_heads, 2, block_size,
                                         dtype=torch.uint8, device=device)
         self.free_blocks: list[int] = list(range(num_blocks))

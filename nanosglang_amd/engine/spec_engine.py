@@ -221,7 +221,8 @@ class SpecEngine:
         self.seed = seed
         self.device = model.device
         self.bm = BlockManager(num_blocks, block_size, model.num_layers, c.num_key_value_heads,
-                               c.head_dim, dtype=kernels._kv_dtype(kv_dtype), device=self.device)
+                               c.head_dim, dtype=kernels._kv_dtype(kv_dtype), device=self.device,
+                               row_scales=kernels._kv_dtype(kv_dtype) == kernels.FP8)
         self.kv = PagedKVCache(self.bm)
         self.P = block_size
         self.attn_ws = torch.empty(workspace_bytes, dtype=torch.uint8, device=self.device)

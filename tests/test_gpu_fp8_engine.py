@@ -15,7 +15,7 @@ Hq, Hkv, D, P = 4, 2, 64, 16          # TINY's
 
 def _manager(blocks=64, layers=4):
     from nanosglang_amd.engine.paged_kv_cache import BlockManager, PagedKVCache
-    bm = BlockManager(blocks, P, layers, Hkv, D, FP8, "cuda")
+    bm = BlockManager(blocks, P, layers, Hkv, D, FP8, "cuda", row_scales=True)
     return bm, PagedKVCache(bm)
 
 

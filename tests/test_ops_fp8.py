@@ -72,7 +72,7 @@ def test_operators_refuse_host_tensors(name):
 
 
 def test_block_manager_of_an_8_bit_pool():
-    bm = BlockManager(6, 16, 3, 2, 64, FP8, "cpu")
+    bm = BlockManager(6, 16, 3, 2, 64, FP8, "cpu", row_scales=True)
     assert [t.dtype for t in bm.caches] == [FP8, FP8, torch.uint8]
     assert bm.kv_scale.shape == (3, 6, 2, 2, 16)
     assert bm.memory_bytes == 3 * 6 * 16 * 2 * (2 * 64 + 2)
@@ -82,8 +82,14 @@ def test_block_manager_of_an_8_bit_pool():
         bm.write_kv(t.block_indices[0], 0, 3, z, z)
     with pytest.raises(ValueError, match="do not fit"):          # the next block's slots
         bm.write_kv(t.block_indices[0], 0, 12, z, z)
-    plain = BlockManager(6, 16, 3, 2, 64, torch.bfloat16, "cpu")
-    assert plain.kv_scale is None and len(plain.caches) == 2
+    for dtype in (torch.bfloat16, FP8):                          # caches of any type, as before
+        plain = BlockManager(6, 16, 3, 2, 64, dtype, "cpu")
+        plain.write_kv(2, 1, 3, z + 1, z + 2)
+        k, v = plain.read_kv([2], 1, 8)
+        assert plain.kv_scale is None and len(plain.caches) == 2
+        assert (k[:, 3:].float() == 1).all() and (v[:, 3:].float() == 2).all()
+    with pytest.raises(ValueError, match="row_scales"):
+        BlockManager(6, 16, 3, 2, 64, torch.bfloat16, "cpu", row_scales=True)
 
 
 def test_bf16_writers_refuse_the_8_bit_pool(monkeypatch):
