@@ -50,7 +50,7 @@ enum {
 const char* nsg_last_error(void);
 /* ABI version of this header (NSG_ABI_VERSION). */
 int32_t nsg_abi_version(void);
-#define NSG_ABI_VERSION 23
+#define NSG_ABI_VERSION 24
 
 /* ------------------------------------------------------------------------
  * Verify attention: ragged multi-query attention over the paged KV cache
@@ -139,12 +139,25 @@ int32_t nsg_attn_run(const nsg_attn_plan_t* plan, const int32_t* work_d,
                      int32_t page_size, int32_t num_pages, float sm_scale, int32_t causal,
                      void* workspace, int64_t workspace_bytes, nsg_stream_t stream);
 
-/* nsg_attn_run over the 8-bit pool: the plans are the same (nsg_attn_plan /
- * nsg_attn_plan_fixed), k_cache / v_cache hold e4m3 codes and kv_scale their
+/* nsg_attn_run over the 8-bit pool.  Any plan serves either pool; these two,
+ * arguments as nsg_attn_plan's and nsg_attn_plan_fixed's (whose capacity they
+ * fit), cut long contexts into items of twice the tokens.  k_cache / v_cache hold e4m3 codes and kv_scale their
  * E8M0 scales.  Q stays bf16 and unquantised, codes and scales are exact in
  * bf16: the outputs are those of attention over the values that the pool
  * stands for, with the probabilities rounded to bf16 after V's scale is
  * applied.  q, out and the caches must be 16-byte aligned. */
+int32_t nsg_attn_plan_fp8(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
+                          const int32_t* kv_last_page_len_h, int32_t batch,
+                          int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                          int32_t page_size, int32_t causal, int32_t num_cus, int32_t* work_h,
+                          int32_t work_capacity, nsg_attn_plan_t* plan);
+int32_t nsg_attn_plan_fixed_fp8(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
+                                const int32_t* kv_last_page_len_h, int32_t batch,
+                                int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+                                int32_t page_size, int32_t causal, int32_t num_cus,
+                                int32_t max_q_len, int32_t max_kv_len, int32_t max_work,
+                                int32_t max_merge, int32_t* work_h, int32_t work_capacity,
+                                nsg_attn_plan_t* plan);
 int32_t nsg_attn_run_fp8(const nsg_attn_plan_t* plan, const int32_t* work_d, const void* q,
                          const void* k_cache, const void* v_cache, const void* kv_scale, void* out,
                          const int32_t* kv_indices, int32_t page_size, int32_t num_pages,

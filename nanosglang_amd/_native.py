@@ -13,7 +13,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libnsg_spec.so")
 
 NSG_ATTN_WORK_INTS = 8
-ABI_VERSION = 23
+ABI_VERSION = 24
 
 i32, i64, u32, u64, f32 = C.c_int32, C.c_int64, C.c_uint32, C.c_uint64, C.c_float
 vp = C.c_void_p
@@ -73,6 +73,10 @@ SIGNATURES = {
                                  i32, vp, vp, vp, vp, i64, vp, vp]),
     "nsg_attn_run": (i32, [C.POINTER(AttnPlan), vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i32,
                            f32, i32, vp, i64, vp]),
+    "nsg_attn_plan_fp8": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, i32,
+                                C.POINTER(AttnPlan)]),
+    "nsg_attn_plan_fixed_fp8": (i32, [vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32,
+                                      i32, i32, vp, i32, C.POINTER(AttnPlan)]),
     "nsg_attn_run_fp8": (i32, [C.POINTER(AttnPlan), vp, vp, vp, vp, vp, vp, vp, i32, i32, f32,
                                i32, vp, i64, vp]),
     "nsg_kv_write_fp8": (i32, [vp, i64, vp, i64, vp, i32, vp, vp, vp, i32, i32, i32, i64, vp]),

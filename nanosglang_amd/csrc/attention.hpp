@@ -92,6 +92,17 @@ __device__ __forceinline__ int swz_v(int t) {
 }
 
 
+// A planner called from the C ABI, which no C++ exception crosses.
+template <typename F>
+int32_t guarded(F&& f) {
+  try {
+    return f();
+  } catch (...) {
+    set_error("out of host memory while planning");
+    return NSG_ERR_ARG;
+  }
+}
+
 // The attention planner behind nsg_attn_plan (fixed_work < 0) and
 // nsg_attn_plan_fixed (its max_work, max_merge, max_q_len, max_kv_len); regime: 1
 // several KV groups per workgroup, 0 one, -1 the planner's own choice.

@@ -363,16 +363,6 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
   return NSG_OK;
 }
 
-template <typename F>
-int32_t guarded(F&& f) {  // no C++ exception crosses the C ABI
-  try {
-    return f();
-  } catch (...) {
-    set_error("out of host memory while planning");
-    return NSG_ERR_ARG;
-  }
-}
-
 }  // namespace
 }  // namespace nsg
 

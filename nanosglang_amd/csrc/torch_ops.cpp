@@ -20,7 +20,8 @@
 //   nsg::kv_write, nsg::rope_kv_write
 //                               K / V rows (after RoPE) into flat KV slots
 //   nsg::kv_write_fp8, nsg::rope_kv_write_fp8, nsg::kv_read_fp8,
-//   nsg::verify_attention_fp8, nsg::verify_attention_run_fp8
+//   nsg::verify_attention_fp8, nsg::verify_attention_plan_fp8,
+//   nsg::verify_attention_run_fp8
 //                               the same over the 8-bit pool, and its rows back
 //   nsg::shared_prefix_attention  groups of requests behind common prefixes
 //
@@ -125,12 +126,11 @@ int64_t work_bound(const int32_t* qo, const int32_t* kvp, const int32_t* last, i
   return std::max<int64_t>(1, bound);
 }
 
-std::tuple<Tensor, Tensor> verify_attention_plan(const Tensor& qo_indptr,
-                                                 const Tensor& paged_kv_indptr,
-                                                 const Tensor& paged_kv_last_page_len,
-                                                 int64_t num_qo_heads, int64_t num_kv_heads,
-                                                 int64_t head_dim, int64_t page_size,
-                                                 bool causal, int64_t num_cus) {
+std::tuple<Tensor, Tensor> plan_with(decltype(&nsg_attn_plan) planner, const Tensor& qo_indptr,
+                                     const Tensor& paged_kv_indptr,
+                                     const Tensor& paged_kv_last_page_len, int64_t num_qo_heads,
+                                     int64_t num_kv_heads, int64_t head_dim, int64_t page_size,
+                                     bool causal, int64_t num_cus) {
   const Tensor qo = host_i32(qo_indptr), kvp = host_i32(paged_kv_indptr),
                last = host_i32(paged_kv_last_page_len);
   const int64_t B = qo.numel() - 1;
@@ -141,18 +141,29 @@ std::tuple<Tensor, Tensor> verify_attention_plan(const Tensor& qo_indptr,
                                  page_size);
   Tensor work = at::zeros({cap * NSG_ATTN_WORK_INTS}, at::TensorOptions().dtype(at::kInt));
   nsg_attn_plan_t pl{};
-  check_status(nsg_attn_plan(qo.data_ptr<int32_t>(), kvp.data_ptr<int32_t>(),
-                             last.data_ptr<int32_t>(), static_cast<int32_t>(B),
-                             static_cast<int32_t>(num_qo_heads),
-                             static_cast<int32_t>(num_kv_heads), static_cast<int32_t>(head_dim),
-                             static_cast<int32_t>(page_size), causal ? 1 : 0,
-                             static_cast<int32_t>(num_cus), work.data_ptr<int32_t>(),
-                             static_cast<int32_t>(cap), &pl),
+  check_status(planner(qo.data_ptr<int32_t>(), kvp.data_ptr<int32_t>(), last.data_ptr<int32_t>(),
+                       static_cast<int32_t>(B), static_cast<int32_t>(num_qo_heads),
+                       static_cast<int32_t>(num_kv_heads), static_cast<int32_t>(head_dim),
+                       static_cast<int32_t>(page_size), causal ? 1 : 0,
+                       static_cast<int32_t>(num_cus), work.data_ptr<int32_t>(),
+                       static_cast<int32_t>(cap), &pl),
                "nsg_attn_plan");
   const int64_t n = static_cast<int64_t>(pl.num_work + pl.num_merge) * NSG_ATTN_WORK_INTS;
   return {make_record(pl, qo.data_ptr<int32_t>()[B], kvp.data_ptr<int32_t>()[B], B),
           work.narrow(0, 0, n).clone()};
 }
+
+template <decltype(&nsg_attn_plan) PLANNER>
+std::tuple<Tensor, Tensor> attention_plan(const Tensor& qo_indptr, const Tensor& paged_kv_indptr,
+                                          const Tensor& paged_kv_last_page_len,
+                                          int64_t num_qo_heads, int64_t num_kv_heads,
+                                          int64_t head_dim, int64_t page_size, bool causal,
+                                          int64_t num_cus) {
+  return plan_with(PLANNER, qo_indptr, paged_kv_indptr, paged_kv_last_page_len, num_qo_heads,
+                   num_kv_heads, head_dim, page_size, causal, num_cus);
+}
+constexpr auto verify_attention_plan = attention_plan<nsg_attn_plan>;
+constexpr auto verify_attention_plan_fp8 = attention_plan<nsg_attn_plan_fp8>;
 
 void verify_attention_run(const Tensor& plan, const Tensor& work, const Tensor& q,
                           const Tensor& k_cache, const Tensor& v_cache, const Tensor& qo_indptr,
@@ -642,9 +653,10 @@ Tensor verify_attention_fp8(const Tensor& q, const Tensor& k_cache, const Tensor
   require_fp8_pool(k_cache, v_cache, kv_scale, dev);
   TORCH_CHECK_VALUE(q.dim() == 3, "q must be (T, Hq, D)");
   const int64_t D = q.size(2);
-  auto [rec, work_h] = verify_attention_plan(qo_indptr, paged_kv_indptr, paged_kv_last_page_len,
-                                             q.size(1), k_cache.size(2), D, k_cache.size(1),
-                                             causal, kMi355xCus);
+  auto [rec, work_h] = verify_attention_plan_fp8(qo_indptr, paged_kv_indptr,
+                                                 paged_kv_last_page_len, q.size(1),
+                                                 k_cache.size(2), D, k_cache.size(1), causal,
+                                                 kMi355xCus);
   nsg_attn_plan_t pl;
   int64_t total_q, nnz, B;
   read_record(rec, &pl, &total_q, &nnz, &B);
@@ -792,6 +804,10 @@ TORCH_LIBRARY(nsg, m) {
       "Tensor qo_indptr, Tensor paged_kv_indptr, Tensor paged_kv_indices, "
       "Tensor paged_kv_last_page_len, bool causal=True, float? sm_scale=None) -> Tensor");
   m.def(
+      "verify_attention_plan_fp8(Tensor qo_indptr, Tensor paged_kv_indptr, "
+      "Tensor paged_kv_last_page_len, int num_qo_heads, int num_kv_heads, int head_dim, "
+      "int page_size, bool causal=True, int num_cus=256) -> (Tensor, Tensor)");
+  m.def(
       "verify_attention_run_fp8(Tensor plan, Tensor work, Tensor q, Tensor k_cache, "
       "Tensor v_cache, Tensor kv_scale, Tensor paged_kv_indices, float sm_scale, bool causal, "
       "Tensor(a!) workspace, Tensor(b!) out) -> ()");
@@ -805,7 +821,8 @@ TORCH_LIBRARY(nsg, m) {
 
 TORCH_LIBRARY_IMPL(nsg, CUDA, m) {
   m.impl("verify_attention", &verify_attention);
-  m.impl("verify_attention_plan", &verify_attention_plan);
+  m.impl("verify_attention_plan", verify_attention_plan);
+  m.impl("verify_attention_plan_fp8", verify_attention_plan_fp8);
   m.impl("verify_attention_run", &verify_attention_run);
   m.impl("spec_accept", &spec_accept);
   m.impl("sample", &sample);
@@ -820,7 +837,8 @@ TORCH_LIBRARY_IMPL(nsg, CUDA, m) {
 }
 
 TORCH_LIBRARY_IMPL(nsg, CPU, m) {
-  m.impl("verify_attention_plan", &verify_attention_plan);   // the host planner
+  m.impl("verify_attention_plan", verify_attention_plan);
+  m.impl("verify_attention_plan_fp8", verify_attention_plan_fp8);   // the host planner
   m.impl("verify_attention", [](const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                                 const Tensor&, const Tensor&, const Tensor&, bool,
                                 optional<double>) -> Tensor { host_tensors("verify_attention"); });

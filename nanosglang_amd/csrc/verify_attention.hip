@@ -1010,7 +1010,7 @@ int32_t plan_impl(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
                   int32_t num_kv_heads, int32_t head_dim, int32_t page_size, int32_t causal,
                   int32_t num_cus, int32_t* work_h, int32_t work_capacity, int32_t fixed_work,
                   int32_t fixed_merge, int32_t fixed_q_len, int32_t fixed_kv_len,
-                  int32_t regime, nsg_attn_plan_t* plan) {
+                  int32_t regime, bool kv8, nsg_attn_plan_t* plan) {
   NSG_CHECK_ARG(plan && qo_indptr_h && kv_indptr_h && kv_last_page_len_h, "null argument");
   NSG_CHECK_ARG(batch >= 0, "batch %d < 0", batch);
   NSG_CHECK_ARG(num_kv_heads > 0 && num_qo_heads > 0 && num_qo_heads % num_kv_heads == 0,
@@ -1112,6 +1112,13 @@ int32_t plan_impl(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
     const long long tgt = target_items(KS, num_cus, num_kv_heads);
     chunk_it = std::max<long long>((long long)(KS > 1 ? kMinGroupSteps : kMinSplitSteps) * KS,
                                    (total_it + tgt - 1) / tgt);
+    // Twice as long over the 8-bit pool, whose steps are half the bytes (64 x 9
+    // rows over 2048 - 8192 tokens, 32 / 8 heads of 128: 193 -> 179 us; 60 x 1 over
+    // 1000 - 8000, 8 / 1: 59 -> 48), and where every item leaves partial rows of
+    // more than one 16-row tile (96 x 5 rows with 100 - 1000 tokens of their own
+    // behind a prefix: 96.5 -> 91 us; 128 x 5 with 20 - 200, 14 / 2 heads of 64: 30.9
+    // and 32.5).
+    if (KS == 1 && (kv8 || (regime == 0 && T * G > 16))) chunk_it *= 2;
     const long long max_chunk_it =
         std::max<long long>(1, ((long long)(kMaxItemPages - 2) * page_size) / kTokIt);
     chunk_it = std::min(chunk_it, max_chunk_it);
@@ -1301,7 +1308,7 @@ int32_t plan_attn(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
                   nsg_attn_plan_t* plan) {
   return plan_impl(qo_indptr_h, kv_indptr_h, kv_last_page_len_h, batch, num_qo_heads,
                    num_kv_heads, head_dim, page_size, causal, num_cus, work_h, work_capacity,
-                   fixed_work, fixed_merge, fixed_q_len, fixed_kv_len, regime, plan);
+                   fixed_work, fixed_merge, fixed_q_len, fixed_kv_len, regime, false, plan);
 }
 
 }  // namespace nsg
@@ -1313,7 +1320,20 @@ extern "C" int32_t nsg_attn_plan(const int32_t* qo_indptr_h, const int32_t* kv_i
                                  int32_t* work_h, int32_t work_capacity, nsg_attn_plan_t* plan) {
   return plan_impl(qo_indptr_h, kv_indptr_h, kv_last_page_len_h, batch, num_qo_heads,
                    num_kv_heads, head_dim, page_size, causal, num_cus, work_h, work_capacity,
-                   -1, 0, 0, 0, -1, plan);
+                   -1, 0, 0, 0, -1, false, plan);
+}
+
+extern "C" int32_t nsg_attn_plan_fp8(const int32_t* qo_indptr_h, const int32_t* kv_indptr_h,
+                                     const int32_t* kv_last_page_len_h, int32_t batch,
+                                     int32_t num_qo_heads, int32_t num_kv_heads,
+                                     int32_t head_dim, int32_t page_size, int32_t causal,
+                                     int32_t num_cus, int32_t* work_h, int32_t work_capacity,
+                                     nsg_attn_plan_t* plan) {
+  return guarded([&] {
+    return plan_impl(qo_indptr_h, kv_indptr_h, kv_last_page_len_h, batch, num_qo_heads,
+                     num_kv_heads, head_dim, page_size, causal, num_cus, work_h, work_capacity,
+                     -1, 0, 0, 0, -1, true, plan);
+  });
 }
 
 extern "C" int32_t nsg_attn_fixed_capacity(int32_t batch, int32_t max_q_len,
@@ -1347,7 +1367,25 @@ extern "C" int32_t nsg_attn_plan_fixed(const int32_t* qo_indptr_h, const int32_t
                 (kMaxItemPages - 2) * page_size);
   return plan_impl(qo_indptr_h, kv_indptr_h, kv_last_page_len_h, batch, num_qo_heads,
                    num_kv_heads, head_dim, page_size, causal, num_cus, work_h, work_capacity,
-                   max_work, max_merge, max_q_len, max_kv_len, -1, plan);
+                   max_work, max_merge, max_q_len, max_kv_len, -1, false, plan);
+}
+
+extern "C" int32_t nsg_attn_plan_fixed_fp8(
+    const int32_t* qo_indptr_h, const int32_t* kv_indptr_h, const int32_t* kv_last_page_len_h,
+    int32_t batch, int32_t num_qo_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t page_size, int32_t causal, int32_t num_cus, int32_t max_q_len, int32_t max_kv_len,
+    int32_t max_work, int32_t max_merge, int32_t* work_h, int32_t work_capacity,
+    nsg_attn_plan_t* plan) {
+  NSG_CHECK_ARG(max_q_len >= 1 && max_work >= 1 && max_merge >= 0,
+                "max_q_len %d, max_work %d, max_merge %d", max_q_len, max_work, max_merge);
+  NSG_CHECK_ARG(page_size > 0 && max_kv_len <= (kMaxItemPages - 2) * (int64_t)page_size,
+                "max_kv_len %d exceeds one work item's page list (%lld tokens)", max_kv_len,
+                (kMaxItemPages - 2) * (long long)page_size);
+  return guarded([&] {
+    return plan_impl(qo_indptr_h, kv_indptr_h, kv_last_page_len_h, batch, num_qo_heads,
+                     num_kv_heads, head_dim, page_size, causal, num_cus, work_h, work_capacity,
+                     max_work, max_merge, max_q_len, max_kv_len, -1, true, plan);
+  });
 }
 
 extern "C" int32_t nsg_attn_run(const nsg_attn_plan_t* plan, const int32_t* work_d,

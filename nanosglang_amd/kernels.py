@@ -222,12 +222,11 @@ class BatchPrefillWithPagedKVCacheWrapper:
             self._fixed = (mq, mw.value, mm.value)
         mq, mw, mm = self._fixed
         pl = AttnPlan()
-        check(lib.nsg_attn_plan_fixed(qo_h.ctypes.data, kvp_h.ctypes.data, last_h.ctypes.data, B,
-                                      num_qo_heads, num_kv_heads, head_dim_qk, page_size,
-                                      1 if causal else 0, self._num_cus, mq, self._fixed_kv,
-                                      mw, mm,
-                                      self._work_h.ctypes.data, self._work_h.shape[0],
-                                      C.byref(pl)), "nsg_attn_plan_fixed")
+        fn = lib.nsg_attn_plan_fixed_fp8 if self._kv_dtype == FP8 else lib.nsg_attn_plan_fixed
+        check(fn(qo_h.ctypes.data, kvp_h.ctypes.data, last_h.ctypes.data, B, num_qo_heads,
+                 num_kv_heads, head_dim_qk, page_size, 1 if causal else 0, self._num_cus, mq,
+                 self._fixed_kv, mw, mm, self._work_h.ctypes.data, self._work_h.shape[0],
+                 C.byref(pl)), "nsg_attn_plan_fixed")
         nnz = int(kvp_h[-1])
         idx_buf = self._gbufs["kv_indices"]
         if nnz > idx_buf.numel():
@@ -334,10 +333,10 @@ class BatchPrefillWithPagedKVCacheWrapper:
             self._work_d = torch.empty(self._work_cap * NSG_ATTN_WORK_INTS, dtype=torch.int32,
                                        device=self._device)
         pl = AttnPlan()
-        rc = lib.nsg_attn_plan(qo_h.ctypes.data, kvp_h.ctypes.data, last_h.ctypes.data, B,
-                               num_qo_heads, num_kv_heads, head_dim_qk, page_size,
-                               1 if causal else 0, self._num_cus, self._work_h.ctypes.data,
-                               self._work_cap, C.byref(pl))
+        fn = lib.nsg_attn_plan_fp8 if self._kv_dtype == FP8 else lib.nsg_attn_plan
+        rc = fn(qo_h.ctypes.data, kvp_h.ctypes.data, last_h.ctypes.data, B, num_qo_heads,
+                num_kv_heads, head_dim_qk, page_size, 1 if causal else 0, self._num_cus,
+                self._work_h.ctypes.data, self._work_cap, C.byref(pl))
         check(rc, "nsg_attn_plan")
         n = (pl.num_work + pl.num_merge) * NSG_ATTN_WORK_INTS
         if n:

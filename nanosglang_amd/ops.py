@@ -32,8 +32,8 @@ nano_sglang/model/causal_lm.py:340), the KV ``index_put`` (causal_lm.py:
 ``nsg::kv_write_fp8``, ``nsg::rope_kv_write_fp8``, ``nsg::kv_read_fp8``
     the same into the 8-bit pool (``kernels.kv_write_fp8``), and rows of it as
     bf16.
-``nsg::verify_attention_fp8``, ``nsg::verify_attention_run_fp8``
-    attention over the 8-bit pool, planned by ``nsg::verify_attention_plan``.
+``nsg::verify_attention_fp8``, ``nsg::verify_attention_plan_fp8``, ``nsg::verify_attention_run_fp8``
+    attention over the 8-bit pool, as the three above.
 ``nsg::shared_prefix_attention``
     plan + run of ``kernels.SharedPrefixAttentionWrapper`` (either pool:
     ``kv_scale`` None is bf16); it synchronises as ``nsg::verify_attention``
@@ -101,6 +101,7 @@ def _(q, k_cache, v_cache, qo_indptr, paged_kv_indptr, paged_kv_indices,
 
 
 @torch.library.register_fake("nsg::verify_attention_plan")
+@torch.library.register_fake("nsg::verify_attention_plan_fp8")
 def _(qo_indptr, paged_kv_indptr, paged_kv_last_page_len, num_qo_heads, num_kv_heads,
       head_dim, page_size, causal=True, num_cus=256):
     n = torch.library.get_ctx().new_dynamic_size()

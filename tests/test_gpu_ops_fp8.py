@@ -73,7 +73,7 @@ def test_attention_equals_the_wrapper_and_replays(Hq, Hkv, D):
     w.plan(qo, ptr, idx, last, Hq, Hkv, D, P, kv_data_type=FP8)
     want = w.run(q, (kc, vc), kv_scale=sc)
     assert torch.equal(OP.verify_attention_fp8(q, kc, vc, sc, qo_d, ptr, idx, last), want)
-    rec, work = OP.verify_attention_plan(torch.from_numpy(qo), ptr.cpu(), last.cpu(), Hq, Hkv, D, P)
+    rec, work = OP.verify_attention_plan_fp8(torch.from_numpy(qo), ptr.cpu(), last.cpu(), Hq, Hkv, D, P)
     ws = torch.zeros(max(1, ops.plan_workspace_bytes(rec)), dtype=torch.uint8, device="cuda")
     out, work, q_s = torch.empty_like(q), work.cuda(), q.clone()
     run = lambda: OP.verify_attention_run_fp8(rec, work, q_s, kc, vc, sc, idx, D ** -0.5, True, ws,

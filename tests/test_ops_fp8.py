@@ -18,6 +18,9 @@ PAGES = ["paged_kv_indptr", "paged_kv_indices", "paged_kv_last_page_len"]
     ("rope_kv_write_fp8", ["qkv", "num_qo_heads", "num_kv_heads", "head_dim", "positions",
                            "cos_table", "sin_table", "slots"] + POOL, set(POOL)),
     ("verify_attention_fp8", ["q"] + POOL + ["qo_indptr"] + PAGES + ["causal", "sm_scale"], set()),
+    ("verify_attention_plan_fp8", ["qo_indptr", "paged_kv_indptr", "paged_kv_last_page_len",
+                                   "num_qo_heads", "num_kv_heads", "head_dim", "page_size",
+                                   "causal", "num_cus"], set()),
     ("verify_attention_run_fp8", ["plan", "work", "q"] + POOL + [
         "paged_kv_indices", "sm_scale", "causal", "workspace", "out"], {"workspace", "out"}),
     ("shared_prefix_attention", ["q"] + POOL + [
@@ -31,6 +34,27 @@ def test_schemas_and_kernels(name, args, written):
             if a.alias_info is not None and a.alias_info.is_write} == written
     for key in ("CUDA", "CPU"):
         assert torch._C._dispatch_has_kernel_for_dispatch_key(f"nsg::{name}", key), key
+
+
+@pytest.mark.parametrize("batch,q,lo,hi", [(64, 9, 2048, 8192), (300, 1, 500, 4000),
+                                           (4, 5, 100, 640)])
+def test_plans_of_the_8_bit_pool_cut_contexts_half_as_often(batch, q, lo, hi):
+    """The same tiles, in fewer and longer items; short contexts (several KV
+    groups a workgroup) are not cut differently."""
+    rng = np.random.default_rng(batch)
+    kv = rng.integers(lo, hi, batch)
+    ptr = np.concatenate([[0], np.cumsum(-(-kv // 16))]).astype(np.int32)
+    args = [torch.from_numpy(x) for x in ((np.arange(batch + 1) * q).astype(np.int32), ptr,
+                                          ((kv - 1) % 16 + 1).astype(np.int32))]
+    plans = [ops.plan_from_record(op(*args, 32, 8, 128, 16)[0])[0] for op in (
+        torch.ops.nsg.verify_attention_plan, torch.ops.nsg.verify_attention_plan_fp8)]
+    a, b = plans
+    assert (a.num_groups, a.row_tiles, a.kv_groups) == (b.num_groups, b.row_tiles, b.kv_groups)
+    if a.kv_groups > 1:
+        assert bytes(a) == bytes(b)
+    else:
+        assert batch <= b.num_work < a.num_work and b.max_splits < a.max_splits
+        assert b.workspace_bytes < a.workspace_bytes
 
 
 def _args(device):
