@@ -41,7 +41,8 @@ struct MergeParams {
 };
 
 // Merge item: [first query token, query tokens, first own item, own splits,
-// the group's first prefix item, its splits, its first query token, -].  A piece
+// the group's first prefix item, its shares, its first query token, its prefix
+// tiles]; a tile's shares are that many items apart.  A piece
 // is 8 columns of a row; its partials are folded in batches of kBatch, whose
 // loads are in flight together, by one lane, or (LANES = 4, few pieces: memory
 // round trips count) every fourth by each of the lanes l, l + 16, l + 32, l + 48 of
@@ -70,8 +71,8 @@ __global__ __launch_bounds__(kThreads) void prefix_merge_kernel(MergeParams p) {
   const float* own = p.own + (((size_t)wi0 * p.Hkv + h) * p.own_rows + row) * PSTRIDE;
   const size_t own_step = (size_t)p.Hkv * p.own_rows * PSTRIDE;
   const float* pre =
-      p.prefix + (((size_t)(pw0 + tile * pns) * p.Hkv + h) * p.prefix_rows + prow) * PSTRIDE;
-  const size_t pre_step = (size_t)p.Hkv * p.prefix_rows * PSTRIDE;
+      p.prefix + (((size_t)(pw0 + tile) * p.Hkv + h) * p.prefix_rows + prow) * PSTRIDE;
+  const size_t pre_step = (size_t)mw[7] * p.Hkv * p.prefix_rows * PSTRIDE;
   float M = kMaskVal, lsum = 0.f;
   float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   const int n = ns + pns;
@@ -238,9 +239,10 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
     own_items += w[1] > 0;
     own_longest = std::max(own_longest, n);
   }
+  // Shares of `chunk` steps; with `rest`, the last one of that many instead.
   struct Choice {
     double us = -1;
-    int64_t chunk = 1;
+    int64_t chunk = 1, rest = 0;
   };
   auto choose = [&](int rows, bool joint) {
     Choice best;
@@ -259,7 +261,23 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
           (joint ? launch_us(fit, (items + own_items) * Hkv, (double)(steps + own_steps) * Hkv,
                              std::max(c, own_longest), false, num_cus)
                  : launch_us(fit, items * Hkv, (double)steps * Hkv, c, num_groups == 1, num_cus));
-      if (best.us < 0 || us < best.us) best = {us, c};
+      if (best.us < 0 || us < best.us) best = {us, c, 0};
+    }
+    // One group's tiles of a whole CU each, n shares of which leave an eighth of
+    // the CUs or more without any: those take a last, short share of every tile, r
+    // one after the other in the time of one long one (2304 rows behind 8192
+    // tokens, 8-bit pool, 9 x 8 tiles: 108 -> 99 us and a merge of 11.4 for 10.2;
+    // 45 other batches 1 - 1.19 times as fast, 1.06 in the mean; 660 rows behind
+    // 7700, where a sixteenth is idle, 56 -> 62).
+    const int64_t tiles = num_groups == 1 ? tiles_of(0, T) * Hkv : 0, n = tiles ? num_cus / tiles : 0;
+    if (!joint && !sz.fixed && rows == 256 && n >= fewest && (num_cus - n * tiles) * 8 >= num_cus) {
+      const int64_t r = (tiles + num_cus - n * tiles - 1) / (num_cus - n * tiles);
+      const double again = (r - 1) * fit.start / fit.step;  // steps' worth of their starts
+      const int64_t b = (int64_t)((longest - n * again) / (n * r + 1));
+      const int64_t c = (longest - b + n - 1) / n;
+      const double us = partials_us(tiles * (n + 1), real_rows, head_dim, (int)n + 1) + fit.start +
+                        fit.step * std::max((double)c, r * b + again);
+      if (b >= 1 && us < best.us) best = {us, c, b};
     }
     return best;
   };
@@ -279,20 +297,20 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
       choice = joint;
     }
   }
-  const int64_t chunk = choice.chunk;
   const int T = std::max(1, rows / G);
   const int own_rows = one_launch ? rows : op.row_tiles * 16;
   std::vector<int32_t> pre;
   std::vector<int> first(num_groups), splits(num_groups);
   for (int g = 0; g < num_groups; ++g) {
     const int len = prefix_len(g), tiles = tiles_of(g, T), q0 = qo[groups[g]], q1 = qo[groups[g + 1]];
-    const int64_t steps = steps_of(g);
-    const int ns = (int)((steps + chunk - 1) / chunk);
+    const int64_t steps = steps_of(g), even = steps - choice.rest;
+    const int n = (int)((even + choice.chunk - 1) / choice.chunk), ns = n + (choice.rest > 0);
     first[g] = (int)(pre.size() / NSG_ATTN_WORK_INTS);
     splits[g] = ns;
-    for (int t = 0; t < tiles; ++t)
-      for (int s = 0; s < ns; ++s) {
-        const int b = (int)(steps * s / ns) * kStep, e = (int)(steps * (s + 1) / ns) * kStep;
+    for (int s = 0; s < ns; ++s)  // (the short shares last)
+      for (int t = 0; t < tiles; ++t) {
+        const int b = (int)(s < n ? even * s / n : even) * kStep;
+        const int e = (int)(s < n ? even * (s + 1) / n : steps) * kStep;
         pre.insert(pre.end(), {q0 + t * T, std::min(T, q1 - q0 - t * T), kAll, pkv[g], b,
                                std::min(len, e), 2, 0});
       }
@@ -320,7 +338,8 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
     g = (int)(std::upper_bound(groups, groups + num_groups + 1, 0,
                                [&](int, int32_t b) { return qo[b] > w[0]; }) -
               groups) - 1;
-    merge.insert(merge.end(), {w[0], w[1], i + own0, ns, first[g], splits[g], qo[groups[g]], 0});
+    merge.insert(merge.end(), {w[0], w[1], i + own0, ns, first[g], splits[g], qo[groups[g]],
+                             tiles_of(g, T)});
     i += ns;
   }
   const int n_merge = (int)(merge.size() / NSG_ATTN_WORK_INTS);

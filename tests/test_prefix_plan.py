@@ -42,7 +42,7 @@ def _check(pl, items, arrays, q_lens, kv_lens, groups, prefix_lens, G, P, causal
     qo, pptr, ptr = arrays
     T, TP = pl.own.q_tile_tokens, pl.prefix_tile_tokens
     seen = np.zeros(qo[-1], int)
-    for qs, qn, wi0, ns, pw0, pns, g0, _ in merge:
+    for qs, qn, wi0, ns, pw0, pns, g0, tiles in merge:
         if qn == 0:
             continue
         b = int(np.searchsorted(qo, qs, side="right") - 1)
@@ -65,7 +65,8 @@ def _check(pl, items, arrays, q_lens, kv_lens, groups, prefix_lens, G, P, causal
         assert pns > 0 or prefix_lens[g] == 0
         for t in range(qs, qs + qn):                  # where the merge looks each token up
             tile, row = divmod(t - g0, TP)
-            its = pre[pw0 + tile * pns:pw0 + (tile + 1) * pns]
+            assert tile < tiles == -(-(qo[groups[g + 1]] - g0) // TP)
+            its = [pre[pw0 + tile + s * tiles] for s in range(pns)]
             assert all(w[0] == g0 + tile * TP and row < w[1] and w[3] == pptr[g] for w in its)
             assert all(w[2] >= 1 << 29 and w[6] >= 2 for w in its)
             if pns:
@@ -93,6 +94,21 @@ def test_every_row_meets_every_token_once(lib, Hq, Hkv, D, P, cus):
         assert not pl.one_launch or pl.own_rows == pl.prefix_rows
         assert pl.workspace_bytes >= 256 + rows * (pl.own.num_work * pl.own_rows
                                                    + pl.num_prefix_work * pl.prefix_rows)
+
+
+def test_short_shares_for_the_cus_that_even_ones_leave_idle(lib):
+    """64 x 9 rows of 4 queries a KV head are 9 tiles of 256: 8 heads x 9 x 3 long
+    shares, and a short one of each tile for the 40 CUs left, two apiece."""
+    q_lens, kv_lens, groups, prefix = [9] * 64, [200] * 64, [0, 64], [8192]
+    rc, pl, items, arrays = _plan(lib, q_lens, kv_lens, groups, prefix)
+    assert rc == 0 and (pl.prefix_rows, pl.one_launch, pl.num_prefix_work) == (256, 0, 36)
+    _check(pl, items, arrays, q_lens, kv_lens, groups, prefix, 4, 16)
+    steps = (items[1][:, 5] - items[1][:, 4]) // 64
+    assert (steps[27:] * 2 < steps[:27].min()).all() and steps[:27].max() < 43
+    # 8 tiles a head: four even shares for every CU
+    rc, pl, items, arrays = _plan(lib, [8] * 64, kv_lens, groups, prefix)
+    assert rc == 0 and pl.num_prefix_work == 32
+    assert (items[1][:, 5] - items[1][:, 4] == 2048).all()
 
 
 def test_prompts_and_not_causal(lib):
