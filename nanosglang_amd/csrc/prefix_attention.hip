@@ -151,6 +151,20 @@ double launch_us(const TileFit& f, int64_t wgs, double steps, int64_t longest, b
                      f.step * std::max((double)longest, steps / num_cus + 0.3 * longest);
 }
 constexpr double kLaunchGap = 1.5;
+// One launch of tiles of up to 64 rows with one KV group, several workgroups to a
+// CU: the longest item's steps, or the CU's share of all steps (of the prefix, which
+// comes from L2, and of own parts) and a third of the longest item's.
+double shared_us(int head_dim, double steps, double own_steps, int64_t longest, int num_cus) {
+  const bool d64 = head_dim == 64;
+  const double item = (d64 ? 1.27 : 1.84) * longest;
+  const double all = d64 ? 0.8 * steps + 0.6 * own_steps : steps + 1.2 * own_steps;
+  return (d64 ? 6.0 : 11.0) + std::max(item, all / num_cus + 0.35 * item);
+}
+// The own parts' launch, with one KV group.
+double own_us(int head_dim, double own_steps, int64_t longest, int num_cus) {
+  const double step = head_dim == 64 ? 0.8 : 1.2, all = head_dim == 64 ? 0.8 : 1.6;
+  return 4.0 + std::max(step * longest, all * own_steps / num_cus);
+}
 constexpr int kFixedJointRows = 512;  // fixed plans: one launch up to so many rows
 
 struct Sizes {
@@ -213,11 +227,15 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
     own.resize(own.size() * 4);
   }
   // ---- the prefix tiles: steps per item, of the shares that the longest
-  //      prefix can be cut into those with the least estimated time.  Where the
-  //      own parts take several KV groups, the prefix may go with them in one
-  //      launch of that kernel (tiles of at most 64 rows), if that is estimated
-  //      ahead of launches of their own: 32 decode rows of 32 / 8 heads of 128
-  //      behind 4001 tokens 33 -> 24 us without the merge. ----
+  //      prefix can be cut into those with the least estimated time; in a launch of
+  //      their own, or (tiles of at most 64 rows, each of which reads the prefix)
+  //      in one with the own parts, of whichever the estimate is lowest: workgroups
+  //      of several KV groups, one to a CU, where few tiles leave time on the table
+  //      (32 decode rows of 32 / 8 heads of 128 behind 4001 tokens: apart 33 us
+  //      without the merge, joint 24), or of one KV group, several to a CU (128
+  //      decode rows behind 1000: apart 40.6 us, joint 27; behind 12000 67 and 87.
+  //      576 batches of 2 - 320 rows a request group behind 300 - 12000: 1.05 times
+  //      as fast in the mean as with several KV groups only, 0.85 - 1.8). ----
   auto prefix_len = [&](int g) {
     const int np = pkv[g + 1] - pkv[g];
     return np ? (np - 1) * page_size + plast[g] : 0;
@@ -244,7 +262,8 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
     double us = -1;
     int64_t chunk = 1, rest = 0;
   };
-  auto choose = [&](int rows, bool joint) {
+  enum How { Apart, Joint, Shared };  // a launch of its own; with the own parts: in KV groups, in one
+  auto choose = [&](int rows, How how) {
     Choice best;
     const TileFit fit = tile_fit(rows, head_dim);
     const int T = std::max(1, rows / G), real_rows = (int)std::min<int64_t>(rows, most);
@@ -258,9 +277,12 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
       if (sz.fixed && items > sz.max_prefix_work && best.us >= 0) break;
       const double us =
           partials_us(items * Hkv, real_rows, head_dim, (int)n) +
-          (joint ? launch_us(fit, (items + own_items) * Hkv, (double)(steps + own_steps) * Hkv,
-                             std::max(c, own_longest), false, num_cus)
-                 : launch_us(fit, items * Hkv, (double)steps * Hkv, c, num_groups == 1, num_cus));
+          (how == Shared ? shared_us(head_dim, (double)steps * Hkv, (double)own_steps * Hkv,
+                                     std::max(c, own_longest), num_cus)
+           : how == Joint
+               ? launch_us(fit, (items + own_items) * Hkv, (double)(steps + own_steps) * Hkv,
+                           std::max(c, own_longest), false, num_cus)
+               : launch_us(fit, items * Hkv, (double)steps * Hkv, c, num_groups == 1, num_cus));
       if (best.us < 0 || us < best.us) best = {us, c, 0};
     }
     // One group's tiles of a whole CU each, n shares of which leave an eighth of
@@ -270,7 +292,7 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
     // 45 other batches 1 - 1.19 times as fast, 1.06 in the mean; 660 rows behind
     // 7700, where a sixteenth is idle, 56 -> 62).
     const int64_t tiles = num_groups == 1 ? tiles_of(0, T) * Hkv : 0, n = tiles ? num_cus / tiles : 0;
-    if (!joint && !sz.fixed && rows == 256 && n >= fewest && (num_cus - n * tiles) * 8 >= num_cus) {
+    if (how == Apart && !sz.fixed && rows == 256 && n >= fewest && (num_cus - n * tiles) * 8 >= num_cus) {
       const int64_t r = (tiles + num_cus - n * tiles - 1) / (num_cus - n * tiles);
       const double again = (r - 1) * fit.start / fit.step;  // steps' worth of their starts
       const int64_t b = (int64_t)((longest - n * again) / (n * r + 1));
@@ -282,20 +304,32 @@ int32_t plan_impl(const int32_t* qo, const int32_t* groups, int32_t num_groups,
     return best;
   };
   int rows = prefix_rows(most, head_dim);
-  Choice choice = choose(rows, false);
-  bool one_launch = false;
-  if (op.kv_groups > 1) {
-    const int joint_rows =
-        std::max(op.row_tiles * 16, prefix_rows(std::min<int64_t>(most, 64), head_dim));
-    const Choice joint = choose(joint_rows, true);
-    const double own_us = launch_us(tile_fit(16, head_dim), own_items * Hkv,
-                                    (double)own_steps * Hkv, own_longest, false, num_cus);
-    // (a fixed plan's shape must not depend on the lengths of one step)
-    one_launch = sz.fixed ? most <= kFixedJointRows : joint.us < choice.us + own_us + kLaunchGap;
-    if (one_launch) {
-      rows = joint_rows;
-      choice = joint;
-    }
+  Choice choice = choose(rows, Apart);
+  const int joint_rows =
+      std::max(op.row_tiles * 16, prefix_rows(std::min<int64_t>(most, 64), head_dim));
+  const Choice groups_joint = op.kv_groups > 1 ? choose(joint_rows, Joint) : Choice{};
+  const Choice shared = choose(joint_rows, Shared);
+  bool one_launch, share_cus;
+  if (sz.fixed) {  // (a fixed plan's shape must not depend on the lengths of one step)
+    one_launch = most <= kFixedJointRows;
+    share_cus = op.kv_groups == 1 || tiles16 * Hkv > num_cus;
+  } else {
+    const double apart =
+        choice.us + kLaunchGap +
+        (op.kv_groups > 1 ? launch_us(tile_fit(16, head_dim), own_items * Hkv,
+                                      (double)own_steps * Hkv, own_longest, false, num_cus)
+                          : own_us(head_dim, (double)own_steps * Hkv, own_longest, num_cus));
+    // (workgroups of 16 waves, four KV groups of head dim 64, run late by as much)
+    share_cus = op.kv_groups == 1 ||
+                shared.us < groups_joint.us * (head_dim == 64 ? 1.15 : 1.0);
+    // (below 16 tokens a page both launches would be of the one-group kernel)
+    one_launch = longest > 0 && ((rows <= 64 && page_size < 16) ||
+                                 (share_cus ? shared.us : groups_joint.us) < apart);
+  }
+  if (one_launch) {
+    rows = joint_rows;
+    choice = share_cus ? shared : groups_joint;
+    if (share_cus) op.kv_groups = 1;
   }
   const int T = std::max(1, rows / G);
   const int own_rows = one_launch ? rows : op.row_tiles * 16;

@@ -99,12 +99,15 @@ def test_groups_of_all_kinds(heads, P, fp8):
     ((32, 8, 128), 13, 1, 1999, 16, 64),     # ... 52
     ((14, 2, 64), 3, 5, 1111, 16, 64),       # ... 105: two tiles of 64
     ((48, 1, 64), 1, 1, 999, 16, 48),        # ... own tiles taller than 16 rows
-    ((32, 8, 128), 3, 1, 2500, 8, 16),       # small pages: launches of their own
+    ((32, 8, 128), 3, 1, 2500, 8, 16),       # small pages: one KV group
     ((32, 8, 128), 13, 1, 1999, 8, 64),
-    ((14, 2, 64), 3, 5, 1111, 8, 128),       # ... 105 rows: the 128-row tile
-    ((32, 8, 128), 25, 1, 1500, 8, 128),
-    ((32, 8, 128), 30, 9, 1500, 16, 256),    # 1080 rows: 256-row tiles, the last partly filled
-    ((14, 2, 64), 33, 5, 700, 8, 128),       # 1155 rows: 128-row tiles
+    ((14, 2, 64), 3, 5, 1111, 8, 64),
+    ((32, 8, 128), 25, 1, 1500, 8, 64),
+    ((32, 8, 128), 30, 9, 1500, 16, 64),     # 1080 rows, tiles of one KV group
+    ((14, 2, 64), 33, 5, 700, 8, 64),
+    ((14, 2, 64), 33, 5, 9000, 8, 128),      # launches of their own: 1155 rows, 128-row tiles
+    ((32, 8, 128), 28, 1, 9000, 1, 128),     # ... 112 rows
+    ((32, 8, 128), 30, 9, 5000, 16, 256),    # 1080 rows: 256-row tiles, the last partly filled
 ])
 def test_tile_shapes(heads, n, q, prefix, P, rows, fp8):
     rng = np.random.default_rng(n)
@@ -112,7 +115,7 @@ def test_tile_shapes(heads, n, q, prefix, P, rows, fp8):
              prefix=[prefix])
     pl = _case(n, c, heads, P, fp8).plan_info
     assert pl.prefix_rows == rows
-    assert pl.one_launch == (P == 16 and rows <= 64)
+    assert pl.one_launch == (rows <= 64)
 
 
 @pytest.mark.parametrize("fp8", [False, True])
@@ -190,7 +193,7 @@ def test_agrees_with_the_per_request_wrapper(fp8):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
-@pytest.mark.parametrize("max_kv_len,Hq", [(0, 14), (800, 14), (800, 4)])
+@pytest.mark.parametrize("max_kv_len,Hq", [(0, 14), (800, 14), (800, 4), (0, 28), (800, 28)])
 def test_graph_mode_replays_after_each_plan(fp8, max_kv_len, Hq):
     """One captured run; requests grow, leave and change groups between the
     replays; rows past the plan's stay as they were."""
@@ -226,7 +229,8 @@ def test_graph_mode_replays_after_each_plan(fp8, max_kv_len, Hq):
         graph.replay()
         torch.cuda.synchronize()
         assert w.check_flags() == 0
-        assert w.plan_info.one_launch == (max_kv_len > 0)    # with the own parts
+        assert w.plan_info.one_launch == (Hq < 28)           # up to 512 rows
+        assert (w.plan_info.own.kv_groups > 1) == (max_kv_len > 0)
         fc.check(out[:n], *_want(q[:n], c, ptabs, tabs, k, v))
         assert (out[n:] == 9.0).all()
 

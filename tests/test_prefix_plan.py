@@ -111,6 +111,21 @@ def test_short_shares_for_the_cus_that_even_ones_leave_idle(lib):
     assert (items[1][:, 5] - items[1][:, 4] == 2048).all()
 
 
+@pytest.mark.parametrize("n,q,prefix,P,one_launch,kv_groups,rows", [
+    (3, 1, 2500, 16, 1, 2, 16), (32, 1, 4001, 16, 1, 2, 64),   # few tiles: KV groups
+    (128, 1, 400, 16, 1, 1, 64), (32, 5, 500, 16, 1, 1, 64),   # many, a short prefix
+    (128, 1, 20000, 16, 0, 1, 256), (30, 9, 5000, 16, 0, 1, 256), (28, 1, 9000, 1, 0, 1, 128),
+    (3, 1, 2500, 8, 1, 1, 16),                                 # pages of less than 16 tokens
+    (64, 9, 0, 16, 0, 1, 256),                                 # no prefix
+])
+def test_which_launches(lib, n, q, prefix, P, one_launch, kv_groups, rows):
+    q_lens, kv_lens = [q] * n, [q + 100] * n
+    rc, pl, items, arrays = _plan(lib, q_lens, kv_lens, [0, n], [prefix], P=P)
+    assert rc == 0
+    assert (pl.one_launch, pl.own.kv_groups, pl.prefix_rows) == (one_launch, kv_groups, rows)
+    _check(pl, items, arrays, q_lens, kv_lens, [0, n], [prefix], 4, P)
+
+
 def test_prompts_and_not_causal(lib):
     q_lens, kv_lens = [1000, 900, 1100], [1000, 1900, 1100]
     rc, pl, items, arrays = _plan(lib, q_lens, kv_lens, [0, 3], [700])
@@ -150,8 +165,7 @@ def test_fixed_plans_keep_one_grid(lib, Hq, Hkv, D, P, max_kv, small):
             used = np.flatnonzero(part[:, 1])
             assert not part[used[-1] + 1 if len(used) else 0:].any()
     assert len(shapes) == 1
-    assert pl.one_launch == (B * mq * Hq // Hkv <= 512 and max_kv > 0 and P >= 16
-                             and pl.own.kv_groups > 1)
+    assert pl.one_launch == (B * mq * Hq // Hkv <= 512)
     rc, *_ = _plan(lib, [1] * 13, [5] * 13, [0, 13], [10], Hq, Hkv, D, P, fixed=fixed)
     assert rc == 1 and b"exceeds" in lib.nsg_last_error()
 
