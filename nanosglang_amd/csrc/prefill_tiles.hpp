@@ -18,8 +18,9 @@
 // pass over K and goes through its steps once more.  Dropping the running maximum
 // (16 max3, a swap, 64 multiplies or, around a branch, as many register moves of
 // the accumulators per step) measured at 4 x 1000-token chunks over 2048 - 8192,
-// 32 / 8 heads of 128, a kernel alone, from 413 to 386 us (pass after pass 326 us,
-// 0.87 PFLOP/s of the causal products).
+// 32 / 8 heads of 128, a kernel alone, from 413 to 386 us.  Pass after pass 318 us now,
+// 0.89 PFLOP/s of the causal products: matrix cores 37 % busy, vector ALU 38 %,
+// LDS 37 %, their phases a third overlapped.
 #pragma once
 
 #include "attention.hpp"
@@ -51,6 +52,20 @@ __device__ __forceinline__ float sum_xor32(float x) {
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
                                                   false);
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// The order of N products, each of which takes READS reads from LDS, in what was
+// scheduled since the last barrier: the reads of AHEAD products first, then a
+// product and the reads of a later one in turn, so that a read's latency passes
+// under AHEAD products (4 x 1000-token chunks over 2048 - 8192, 32 / 8 heads of 128:
+// 331 us with each product behind its own reads, 318 with four ahead, 320 with six).
+template <int N, int READS, int AHEAD, int I = 0>
+__device__ __forceinline__ void feed() {
+  constexpr int kMfma = 0x8, kLdsRead = 0x100;
+  if constexpr (I == 0) __builtin_amdgcn_sched_group_barrier(kLdsRead, READS * AHEAD, 0);
+  __builtin_amdgcn_sched_group_barrier(kMfma, 1, 0);
+  if constexpr (I + AHEAD < N) __builtin_amdgcn_sched_group_barrier(kLdsRead, READS, 0);
+  if constexpr (I + 1 < N) feed<N, READS, AHEAD, I + 1>();
 }
 
 // Ring slots.  Two wave groups (head dim 128, 8 waves): four, a slot is read
@@ -229,18 +244,20 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void attn_tile_kernel(Att
   u32x4 pf[4];       // P^T of it in bf16: one B operand per 16 tokens
   auto qk = [&](int slot) {
     const char* Kt = reinterpret_cast<const char*>(&ring[slot][0][0]);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      floatx16 acc;
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) acc[i] = 0.f;
+      for (int i = 0; i < 16; ++i) sacc[s][i] = 0.f;
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
         const bf16x8 kf = *reinterpret_cast<const bf16x8*>(Kt + 32 * s * D * 2 + (koff ^ (32 * c)));
-        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[c], acc, 0, 0, 0);
+        sacc[s] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[c], sacc[s], 0, 0, 0);
       }
-      sacc[s] = acc;
-    }
+    feed<2 * KC, 1, 4>();
+    __builtin_amdgcn_sched_barrier(0);
   };
   auto mask = [&](int t0) {
 #pragma unroll
@@ -294,6 +311,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void attn_tile_kernel(Att
   };
   auto pv_mul = [&](int slot) {  // O^T += V^T P^T
     const char* Vt = reinterpret_cast<const char*>(&ring[slot][1][0]);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
 #pragma unroll
@@ -307,6 +325,8 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void attn_tile_kernel(Att
             __builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, pf[m]), oacc[dt], 0, 0, 0);
       }
     }
+    feed<4 * DT, 2, 4>();
+    __builtin_amdgcn_sched_barrier(0);
   };
   // A workgroup-wide phase boundary: every LDS access of this wave has
   // completed, nothing moves across.
