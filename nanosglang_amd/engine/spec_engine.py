@@ -220,6 +220,8 @@ class SpecEngine:
         self.filtered = not self.greedy and (self.top_k > 0 or self.top_p < 1.0)
         self.seed = seed
         self.device = model.device
+        # kv_dtype: torch.bfloat16, or torch.float8_e4m3fn for the 8-bit pool (half
+        # the bytes; rows quantised as they are written, kernels.kv_write_fp8)
         self.bm = BlockManager(num_blocks, block_size, model.num_layers, c.num_key_value_heads,
                                c.head_dim, dtype=kernels._kv_dtype(kv_dtype), device=self.device,
                                row_scales=kernels._kv_dtype(kv_dtype) == kernels.FP8)

@@ -327,7 +327,7 @@ class BatchPrefillWithPagedKVCacheWrapper:
     def _plan_dynamic(self, lib, qo_h, kvp_h, last_h, B, num_qo_heads, num_kv_heads,
                       head_dim_qk, page_size, causal) -> AttnPlan:
         bound = attn_work_bound(qo_h, kvp_h, last_h, num_qo_heads, num_kv_heads, page_size)
-        if bound > self._work_cap:
+        if bound > self._work_cap or self._work_d is None:
             self._work_cap = max(bound, 2 * self._work_cap, 64)
             self._work_h = np.zeros(self._work_cap * NSG_ATTN_WORK_INTS, np.int32)
             self._work_d = torch.empty(self._work_cap * NSG_ATTN_WORK_INTS, dtype=torch.int32,
