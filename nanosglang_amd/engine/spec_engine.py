@@ -543,6 +543,7 @@ class SpecEngine:
     # the host gate gives up after this long (a host that never raises the
     # flag, e.g. after an exception, costs this much and sets the gate's error word)
     GATE_TIMEOUT_US = 2_000_000
+    GATE_MAX_SEGS = 8        # ranges one gate copies (csrc/host_gate.hip)
 
     def _graph_for(self, n: int) -> _StepGraph:
         return self._graphs[min(b for b in self._graphs if b >= n)]
@@ -606,7 +607,7 @@ class SpecEngine:
             g.done.value = 0
         if gated:    # the gate also uploads the staging buffer once released
             A = g.arena
-            if pages is None:
+            if pages is None or self.k + 2 > self.GATE_MAX_SEGS:
                 offs, lens, n = ((kernels.C.c_int64 * 1)(0), (kernels.C.c_int64 * 1)(A.nbytes),
                                  1)
             else:    # only the arrays' used prefixes: the pull over PCIe is slow

@@ -260,6 +260,19 @@ def test_engine_over_the_8_bit_pool(graphs):
         assert any(fits)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, FP8])
+def test_pipelined_steps_of_eight_drafts(dtype):
+    """More attention calls than one gate copies ranges for."""
+    from nanosglang_amd.engine.spec_engine import SpecEngine
+    _, gpu = _tiny_models(1.0)
+    rng = np.random.default_rng(5)
+    prompts = [rng.integers(0, 1000, n).tolist() for n in (20, 33)]
+    outs = [SpecEngine(gpu, draft_layers=4, num_speculative=8, num_blocks=64, max_batch=2,
+                       kv_dtype=dtype, pipeline=p).generate(prompts, [40, 25])
+            for p in (True, False)]
+    assert outs[0] == outs[1]
+
+
 @pytest.mark.parametrize("temperature", [0.0, 0.8])
 def test_pipelined_steps_over_the_8_bit_pool(temperature):
     _, gpu = _tiny_models(1.0)
