@@ -50,7 +50,7 @@ enum {
 const char* nsg_last_error(void);
 /* ABI version of this header (NSG_ABI_VERSION). */
 int32_t nsg_abi_version(void);
-#define NSG_ABI_VERSION 24
+#define NSG_ABI_VERSION 25
 
 /* ------------------------------------------------------------------------
  * Verify attention: ragged multi-query attention over the paged KV cache
@@ -275,6 +275,7 @@ typedef struct {
   int32_t indptr_stride;
   int32_t indices_stride;
   int32_t work_stride;
+  int32_t kv8;            /* plans for the 8-bit pool (nsg_attn_plan_fixed_fp8) */
 } nsg_spec_step_bufs_t;
 
 int32_t nsg_spec_step_fill(const int32_t* page_table, int64_t page_table_stride,

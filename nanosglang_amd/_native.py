@@ -13,7 +13,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libnsg_spec.so")
 
 NSG_ATTN_WORK_INTS = 8
-ABI_VERSION = 24
+ABI_VERSION = 25
 
 i32, i64, u32, u64, f32 = C.c_int32, C.c_int64, C.c_uint32, C.c_uint64, C.c_float
 vp = C.c_void_p
@@ -45,6 +45,7 @@ class StepBufs(C.Structure):
         ("verify_pos", vp), ("verify_slot", vp), ("qo_indptr", vp), ("kv_indptr", vp),
         ("kv_last_page_len", vp), ("kv_indices", vp), ("work", vp),
         ("indptr_stride", i32), ("indices_stride", i32), ("work_stride", i32),
+        ("kv8", i32),
     ]
 
 

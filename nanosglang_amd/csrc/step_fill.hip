@@ -215,9 +215,9 @@ int32_t fill_impl(const int32_t* page_table, int64_t page_table_stride, const in
     int32_t rc = nsg_attn_fixed_capacity(S, ql, num_qo_heads, num_kv_heads, num_cus, max_kv_len,
                                          &mw, &mm);
     if (rc != NSG_OK) return rc;
-    rc = nsg_attn_plan_fixed(qo, kvp, last, S, num_qo_heads, num_kv_heads, head_dim, P,
-                             /*causal=*/1, num_cus, ql, max_kv_len, mw, mm, work,
-                             o.work_stride / NSG_ATTN_WORK_INTS, plans + a);
+    rc = (o.kv8 ? nsg_attn_plan_fixed_fp8 : nsg_attn_plan_fixed)(
+        qo, kvp, last, S, num_qo_heads, num_kv_heads, head_dim, P, /*causal=*/1, num_cus, ql,
+        max_kv_len, mw, mm, work, o.work_stride / NSG_ATTN_WORK_INTS, plans + a);
     if (rc != NSG_OK) return rc;
   }
   clear_error();

@@ -150,7 +150,8 @@ class _StepGraph:
         H = A.h
         self.bufs = _native.StepBufs(
             *[H[n].ctypes.data for n in ("tok0", "start", "pos", "slot", "vpos", "vslot", "qo",
-                                         "kvp", "last", "idx", "work")], si, sx, sw)
+                                         "kvp", "last", "idx", "work")], si, sx, sw,
+            eng.bm.kv_scale is not None)
         self.plans = (_native.AttnPlan * (k + 1))()
         D = A.d
         self.pos = [D["pos"][i * bs:(i + 1) * bs] for i in range(k)]

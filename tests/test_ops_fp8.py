@@ -57,6 +57,47 @@ def test_plans_of_the_8_bit_pool_cut_contexts_half_as_often(batch, q, lo, hi):
         assert b.workspace_bytes < a.workspace_bytes
 
 
+def _step_items(lib, kv8):
+    """Work items of each attention call of a filled step, whose plans have to be
+    the pool's own planner's."""
+    import ctypes as C
+    from nanosglang_amd._native import NSG_ATTN_WORK_INTS, AttnPlan
+    from tests import test_step_fill as sf
+    B, k, P, pages = 6, 3, 16, 300
+    tab = np.arange(B * pages, dtype=np.int32).reshape(B, pages)
+    starts = np.asarray([4000, 90, 2500, 17, 4700, 3333], np.int64)
+    npg = ((starts + k + P) // P).astype(np.int32)
+    st = sf._Staging(lib, B, k, 0, ids_stride=B * pages)
+    st.bufs.kv8 = kv8
+    assert sf._fill(lib, st, tab, np.arange(B, dtype=np.int32), npg, starts,
+                    np.zeros(B, np.int64), B, k, P, B * pages - 1, 0) == 0, lib.nsg_last_error()
+    items = []
+    for a in range(k + 1):
+        ql = 1 if a < k else k + 1
+        L = starts + (a + 1 if a < k else k + 1)
+        ptr = np.concatenate([[0], np.cumsum(-(-L // P))]).astype(np.int32)
+        qo, last = (np.arange(B + 1) * ql).astype(np.int32), ((L - 1) % P + 1).astype(np.int32)
+        mw, mm, pl = C.c_int32(0), C.c_int32(0), AttnPlan()
+        assert lib.nsg_attn_fixed_capacity(B, ql, sf.Hq, sf.Hkv, sf.CUS, 0, C.byref(mw),
+                                           C.byref(mm)) == 0
+        n = (mw.value + mm.value) * NSG_ATTN_WORK_INTS
+        work = np.zeros(n, np.int32)
+        plan = lib.nsg_attn_plan_fixed_fp8 if kv8 else lib.nsg_attn_plan_fixed
+        assert plan(qo.ctypes.data, ptr.ctypes.data, last.ctypes.data, B, sf.Hq, sf.Hkv, sf.D, P,
+                    1, sf.CUS, ql, 0, mw.value, mm.value, work.ctypes.data,
+                    n // NSG_ATTN_WORK_INTS, C.byref(pl)) == 0
+        np.testing.assert_array_equal(st.work[a * st.sw:a * st.sw + n], work)
+        assert bytes(st.plans[a]) == bytes(pl)
+        items.append(int((work.reshape(-1, NSG_ATTN_WORK_INTS)[:mw.value, 1] > 0).sum()))
+    assert all(i > B for i in items)                     # split
+    return items
+
+
+def test_step_fill_plans_for_its_pool(lib):
+    """Long contexts (no bound: split plans), in fewer items over the 8-bit pool."""
+    assert all(x < y for x, y in zip(_step_items(lib, 1), _step_items(lib, 0)))
+
+
 def _args(device):
     i32 = dict(dtype=torch.int32, device=device)
     pool = [torch.empty(8, 16, 2, 64, device=device, dtype=FP8) for _ in range(2)]
