@@ -18,9 +18,9 @@
 // pass over K and goes through its steps once more.  Dropping the running maximum
 // (16 max3, a swap, 64 multiplies or, around a branch, as many register moves of
 // the accumulators per step) measured at 4 x 1000-token chunks over 2048 - 8192,
-// 32 / 8 heads of 128, a kernel alone, from 413 to 386 us.  Pass after pass 318 us now,
-// 0.89 PFLOP/s of the causal products: matrix cores 37 % busy, vector ALU 38 %,
-// LDS 37 %, their phases a third overlapped.
+// 32 / 8 heads of 128, a kernel alone, from 413 to 386 us.  Pass after pass 307 us now,
+// 0.93 PFLOP/s of the causal products: matrix cores 39 % busy, vector ALU 40 %,
+// LDS 30 %, their phases a third overlapped.
 #pragma once
 
 #include "attention.hpp"
@@ -54,11 +54,23 @@ __device__ __forceinline__ float sum_xor32(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// V's chunk swizzle: the 32 lanes that one pass of a transposed read serves take
+// four chunks of four neighbouring rows, which fall on 16 different 16-byte bank
+// groups (with the swizzle of prefill_attention.hip on 8: 104,000 of 278,000 LDS
+// cycles a CU were conflicts in the chunks below, 35,000 of 210,000 with this one, and
+// they took 320 us instead of 307).
+template <int D>
+__device__ __forceinline__ int swz_vt(int t) {
+  if constexpr (D == 64) return 4 * ((t >> 1) & 1) + 2 * ((t >> 2) & 1);  // two rows a line
+  return 4 * (t & 3) + 2 * ((t >> 2) & 1);
+}
+
 // The order of N products, each of which takes READS reads from LDS, in what was
 // scheduled since the last barrier: the reads of AHEAD products first, then a
 // product and the reads of a later one in turn, so that a read's latency passes
 // under AHEAD products (4 x 1000-token chunks over 2048 - 8192, 32 / 8 heads of 128:
-// 331 us with each product behind its own reads, 318 with four ahead, 320 with six).
+// 331 us with each product behind its own reads, 318 with four ahead, 320 with six; V as it was
+// swizzled then).
 template <int N, int READS, int AHEAD, int I = 0>
 __device__ __forceinline__ void feed() {
   constexpr int kMfma = 0x8, kLdsRead = 0x100;
@@ -163,7 +175,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void attn_tile_kernel(Att
     const int i = lane & 15, dh = (lane >> 4) & 1;
     const int t = 8 * hh + 4 * g + (i >> 2);
     const int c = 16 * dh + 4 * (i & 3);
-    voff[hh] = 2 * (t * D + (((c >> 3) ^ swz_v<D>(t)) << 3) + (c & 7));
+    voff[hh] = 2 * (t * D + (((c >> 3) ^ swz_vt<D>(t)) << 3) + (c & 7));
   }
 
   const int n_it = (kve - kvb + kStep - 1) / kStep;
@@ -184,7 +196,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void attn_tile_kernel(Att
     const int pc = lane % CPR;
     d_t[i] = t;
     d_k[i] = (pc ^ swz_k<D>(t)) * 16;
-    d_v[i] = (pc ^ swz_v<D>(t)) * 16;
+    d_v[i] = (pc ^ swz_vt<D>(t)) * 16;
     d_lds[i] = t0 * D * 2;
   }
   // tokens past the item's end repeat its last one (masked out)
@@ -234,7 +246,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void attn_tile_kernel(Att
         const fp8_u32x2 va = from_fp8x4(vw[2 * x], vs), vb = from_fp8x4(vw[2 * x + 1], vs);
         *reinterpret_cast<u32x4*>(&ring[slot][0][t * D + ((c + x) ^ swz_k<D>(t)) * 8]) =
             u32x4{ka[0], ka[1], kb[0], kb[1]};
-        *reinterpret_cast<u32x4*>(&ring[slot][1][t * D + ((c + x) ^ swz_v<D>(t)) * 8]) =
+        *reinterpret_cast<u32x4*>(&ring[slot][1][t * D + ((c + x) ^ swz_vt<D>(t)) * 8]) =
             u32x4{va[0], va[1], vb[0], vb[1]};
       }
     }
